@@ -1,0 +1,23 @@
+// Internal launch API of the 8-bit operators (include/rns8/rns8_quant.h).
+// Arguments are validated by the callers in api_quant.cpp; every function
+// enqueues on `stream` and returns the launch's error.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "rns8/rns8_quant.h"
+
+namespace rns8cuda {
+
+cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q,
+                          int64_t ld_q, float* scale, cudaStream_t stream);
+
+uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d, int sm_count);
+cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream);
+
+cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t stream);
+uint64_t residual_norm_backward_scratch_bytes(const rns8_cuda_residual_norm_backward_desc& d, int sm_count);
+cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& d, int sm_count, cudaStream_t stream);
+
+}  // namespace rns8cuda

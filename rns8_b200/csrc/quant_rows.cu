@@ -1,0 +1,91 @@
+// Row quantisation to int8 (include/rns8/rns8_quant.h): one pass over a row
+// held in registers; rows too long for that are read twice.
+#include <algorithm>
+
+#include "quant_common.cuh"
+#include "quant_kernels.hpp"
+
+namespace rns8cuda {
+namespace {
+
+template <typename T, bool ALIGNED, int NV>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, int cols, int64_t ld_x,
+                                                             int8_t* __restrict__ q, int64_t ld_q,
+                                                             float* __restrict__ scale) {
+  __shared__ uint32_t slots[32];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ld_x;
+  float v[NV][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    load8<ALIGNED>(xr, cols, j, blockDim.x, threadIdx.x, v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(v[j][e]));
+  }
+  const RowScale rs = make_row_scale(block_max(top, slots));
+  if (threadIdx.x == 0) scale[row] = rs.scale;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) store_q8<ALIGNED>(q + row * ld_q, cols, j, blockDim.x, threadIdx.x, v[j], rs.inv);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* __restrict__ x, int64_t cols, int64_t ld_x,
+                                                                  int8_t* __restrict__ q, int64_t ld_q,
+                                                                  float* __restrict__ scale) {
+  __shared__ uint32_t slots[32];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ld_x;
+  uint32_t top = 0;
+  for (int64_t i = threadIdx.x; i < cols; i += blockDim.x) top = max(top, magnitude_bits(to_f32(xr[i])));
+  const RowScale rs = make_row_scale(block_max(top, slots));
+  if (threadIdx.x == 0) scale[row] = rs.scale;
+  for (int64_t i = threadIdx.x; i < cols; i += blockDim.x)
+    q[row * ld_q + i] = static_cast<int8_t>(quantize_one(to_f32(xr[i]), rs.inv));
+}
+
+template <typename T>
+cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
+                   cudaStream_t stream) {
+  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(q) % 8 == 0 && ld_q % 8 == 0;
+  const unsigned grid = static_cast<unsigned>(rows);
+  if (cols > 1024 * 8 * 4) {
+    quantize_long_rows_kernel<T><<<grid, 1024, 0, stream>>>(x, cols, ld_x, q, ld_q, scale);
+    return cudaGetLastError();
+  }
+  const int c = static_cast<int>(cols);
+  const int vecs = (c + 7) / 8;
+  auto go = [&](auto nv, auto al) {
+    constexpr int NV = decltype(nv)::value;
+    const int threads = std::max(32, ((vecs + NV - 1) / NV + 31) / 32 * 32);
+    quantize_rows_kernel<T, decltype(al)::value, NV><<<grid, threads, 0, stream>>>(x, c, ld_x, q, ld_q, scale);
+  };
+  auto pick = [&](auto al) {
+    if (vecs <= 1024)
+      go(std::integral_constant<int, 1>{}, al);
+    else
+      go(std::integral_constant<int, 4>{}, al);
+  };
+  if (aligned)
+    pick(std::true_type{});
+  else
+    pick(std::false_type{});
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q,
+                          int64_t ld_q, float* scale, cudaStream_t stream) {
+  switch (x_type) {
+    case RNS8_CUDA_TYPE_BF16:
+      return launch(static_cast<const __nv_bfloat16*>(x), rows, cols, ld_x, q, ld_q, scale, stream);
+    case RNS8_CUDA_TYPE_F16:
+      return launch(static_cast<const __half*>(x), rows, cols, ld_x, q, ld_q, scale, stream);
+    default:
+      return launch(static_cast<const float*>(x), rows, cols, ld_x, q, ld_q, scale, stream);
+  }
+}
+
+}  // namespace rns8cuda
