@@ -59,6 +59,11 @@ bool tma_encode_available();
 // and cells % 128 == 0.
 bool encode_plane_cells(CUtensorMap* map, const void* planes, uint64_t cells, uint32_t plane_count,
                         uint32_t box_rows, uint32_t box_chunks);
+// An int8 matrix of `rows` rows of `cols` bytes, `ld` bytes apart (a multiple
+// of 16, base 16-byte aligned), as a (byte in row, row) tensor with the
+// 128-byte swizzle; a box is 128 bytes of box_rows rows (at most 256). Bytes
+// past the matrix read as zero.
+bool encode_rows_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows);
 cudaError_t tc_wrap64_gemm(const uint8_t* a_limbs, const uint8_t* b_limbs, uint64_t* c, int64_t m, int64_t n,
                            int64_t k, int sm_count, uint32_t* dev_status, cudaStream_t stream);
 

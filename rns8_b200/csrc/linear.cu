@@ -1,96 +1,100 @@
-// Scaled int8 product (include/rns8/rns8_quant.h), first form: 64 x 64 output
-// tiles on the CUDA cores with byte-wise operand loads, right for any
-// alignment.
+// Scaled int8 product (include/rns8/rns8_quant.h): which kernels a call runs,
+// the copies that give unaligned rows a 16-byte start, and the scratch for them.
+#include <algorithm>
+
+#include "linear_internal.hpp"
 #include "quant_common.cuh"
 #include "quant_kernels.hpp"
 
 namespace rns8cuda {
 namespace {
 
-constexpr int TILE = 64, KT = 64;
-
-__device__ __forceinline__ void store_out(void* out, uint32_t type, int64_t i, float v) {
-  if (type == RNS8_CUDA_TYPE_BF16)
-    static_cast<__nv_bfloat16*>(out)[i] = from_f32<__nv_bfloat16>(v);
-  else if (type == RNS8_CUDA_TYPE_F16)
-    static_cast<__half*>(out)[i] = from_f32<__half>(v);
-  else
-    static_cast<float*>(out)[i] = v;
-}
-
-struct LinearArgs {
-  const int8_t* a;
-  const int8_t* w;
-  const float *a_scale, *w_scale, *bias;
-  void* out;
-  int64_t m, n, k, ld_a, ld_w, ld_out;
-  uint32_t out_type, gated;
-};
-
-// 256 threads, 4 x 4 outputs each; a gated tile accumulates both halves.
-__global__ void __launch_bounds__(256) linear_simt_kernel(LinearArgs p) {
-  __shared__ int8_t as[TILE][KT + 4], ws[2][TILE][KT + 4];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * TILE, n0 = static_cast<int64_t>(blockIdx.x) * TILE;
-  const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-  const int halves = p.gated ? 2 : 1;
-  int acc[2][4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += KT) {
-    for (int i = threadIdx.x; i < TILE * KT; i += 256) {
-      const int r = i / KT, c = i % KT;
-      as[r][c] = (m0 + r < p.m && k0 + c < p.k) ? p.a[(m0 + r) * p.ld_a + k0 + c] : 0;
-      for (int h = 0; h < halves; ++h)
-        ws[h][r][c] = (n0 + r < p.n && k0 + c < p.k) ? p.w[(h * p.n + n0 + r) * p.ld_w + k0 + c] : 0;
-    }
-    __syncthreads();
-    for (int c = 0; c < KT; c += 4)
-      for (int h = 0; h < halves; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[h][i][j] = __dp4a(*reinterpret_cast<const int*>(&as[tr + 16 * i][c]),
-                                  *reinterpret_cast<const int*>(&ws[h][tc + 16 * j][c]), acc[h][i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + tr + 16 * i, c = n0 + tc + 16 * j;
-      if (r >= p.m || c >= p.n) continue;
-      float y[2];
-      for (int h = 0; h < halves; ++h) {
-        const int64_t wr = h * p.n + c;
-        y[h] = static_cast<float>(acc[h][i][j]) * p.a_scale[r] * p.w_scale[wr];
-        if (p.bias) y[h] += p.bias[wr];
-      }
-      store_out(p.out, p.out_type, r * p.ld_out + c, p.gated ? y[0] / (1.0f + expf(-y[0])) * y[1] : y[0]);
-    }
-}
-
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
+
+// dst rows (ld a multiple of 16) from src rows of any alignment. Bytes past
+// cols are zero.
+__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ src, int64_t rows, int64_t cols,
+                                                         int64_t ld, int8_t* __restrict__ dst, int64_t ld_dst) {
+  const int64_t per_row = ld_dst / 16, total = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 16; ++b)
+      if (c + b < cols) w[b / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(src[r * ld + c + b])) << (8 * (b % 4));
+    *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+cudaError_t align_rows(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ld_dst,
+                       int sm_count, cudaStream_t stream) {
+  const int64_t chunks = rows * (ld_dst / 16);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((chunks + 255) / 256, sm_count * 16));
+  align_rows_kernel<<<grid, 256, 0, stream>>>(src, rows, cols, ld, dst, ld_dst);
+  return cudaGetLastError();
+}
+
+// What a call needs around its product kernel, and where in scratch.
+struct Steps {
+  LinearArgs args;
+  bool align_w, align_a, quantize, gemv;
+  int64_t ld;
+  uint64_t at_w, at_a, at_scale, bytes;
+};
+Steps plan(const rns8_cuda_linear_desc& d) {
+  Steps s{};
+  s.args = LinearArgs{d.a,      d.w,      d.a_scale,  d.w_scale, d.bias, d.out, d.m, d.n, d.k, d.ld_a, d.ld_w, d.ld_out,
+                      d.a_type, d.out_type, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, false, d.status};
+  const int64_t w_rows = s.args.gated ? 2 * d.n : d.n;
+  s.ld = static_cast<int64_t>(round_up(d.k, 16));
+  s.align_w = !aligned16(d.w, d.ld_w);
+  LinearArgs aligned = s.args;
+  if (s.align_w) aligned.w = nullptr, aligned.ld_w = s.ld;
+  s.gemv = gemv_supported(aligned);
+  s.quantize = !s.gemv && d.a_type != RNS8_CUDA_TYPE_I8;
+  s.align_a = !s.gemv && !s.quantize && !aligned16(d.a, d.ld_a);
+  if (s.align_w) s.bytes = round_up(static_cast<uint64_t>(w_rows) * s.ld, 256);
+  s.at_a = s.bytes;
+  if (s.quantize || s.align_a) s.bytes += round_up(static_cast<uint64_t>(d.m) * s.ld, 256);
+  s.at_scale = s.bytes;
+  if (s.quantize) s.bytes += round_up(4ull * d.m, 256);
+  if (s.bytes) s.bytes += 256;  // the caller's scratch may start anywhere
+  return s;
+}
 
 }  // namespace
 
-uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d, int) {
-  if (d.a_type == RNS8_CUDA_TYPE_I8) return 0;
-  return round_up(static_cast<uint64_t>(d.m) * round_up(d.k, 16), 256) + round_up(4ull * d.m, 256);
-}
+uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d, int) { return plan(d).bytes; }
 
-cudaError_t linear(const rns8_cuda_linear_desc& d, int, cudaStream_t stream) {
-  LinearArgs p{static_cast<const int8_t*>(d.a), d.w, d.a_scale, d.w_scale, d.bias, d.out, d.m, d.n, d.k, d.ld_a, d.ld_w,
-               d.ld_out, d.out_type, d.flags & RNS8_CUDA_LINEAR_GATED};
-  if (d.a_type != RNS8_CUDA_TYPE_I8) {
-    const int64_t ld = static_cast<int64_t>(round_up(d.k, 16));
-    int8_t* q = static_cast<int8_t*>(d.scratch);
-    float* s = reinterpret_cast<float*>(q + round_up(static_cast<uint64_t>(d.m) * ld, 256));
-    const cudaError_t e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, q, ld, s, stream);
+cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream) {
+  Steps s = plan(d);
+  LinearArgs& p = s.args;
+  int8_t* scratch = reinterpret_cast<int8_t*>(round_up(reinterpret_cast<uintptr_t>(d.scratch), 256));
+  cudaError_t e = cudaSuccess;
+  if (s.align_w) {
+    e = align_rows(d.w, p.gated ? 2 * d.n : d.n, d.k, d.ld_w, scratch, s.ld, sm_count, stream);
     if (e != cudaSuccess) return e;
-    p.a = q;
-    p.ld_a = ld;
-    p.a_scale = s;
+    p.w = scratch;
+    p.ld_w = s.ld;
   }
-  const dim3 grid(static_cast<unsigned>((d.n + TILE - 1) / TILE), static_cast<unsigned>((d.m + TILE - 1) / TILE));
-  linear_simt_kernel<<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (s.gemv) return linear_gemv(p, sm_count, stream);
+  if (s.align_a) {
+    e = align_rows(static_cast<const int8_t*>(d.a), d.m, d.k, d.ld_a, scratch + s.at_a, s.ld, sm_count, stream);
+    p.a = scratch + s.at_a;
+    p.ld_a = s.ld;
+  } else if (s.quantize) {
+    float* scale = reinterpret_cast<float*>(scratch + s.at_scale);
+    e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, scratch + s.at_a, s.ld, scale, stream);
+    p.a = scratch + s.at_a;
+    p.ld_a = s.ld;
+    p.a_type = RNS8_CUDA_TYPE_I8;
+    p.a_scale = scale;
+    p.after_quantize = true;
+  }
+  if (e != cudaSuccess) return e;
+  return linear_tc(p, sm_count, stream);
 }
 
 }  // namespace rns8cuda

@@ -1,0 +1,576 @@
+// Scaled int8 product on the tensor cores (tcgen05.mma kind::i8).
+//
+// Two forms, both with TMA rings of 128-byte spans of k (128-byte swizzle, both
+// operands K-major), int32 accumulators in tensor memory and the scales, bias
+// and gate applied on the way out:
+//
+//   tokens on lanes   A persistent kernel, one block per SM: 128 tokens x 256
+//                     weight rows (gated: 128 gate rows and their 128 up rows)
+//                     per tile, two accumulators, so that a tile's epilogue
+//                     runs under the next tile's products. For products with
+//                     about a tile per SM or more.
+//   channels on lanes One tile of 128 output channels (gated: 128 gate and 128
+//                     up rows) x 16..256 tokens per cluster; the blocks of a
+//                     cluster split k and join their exact integer sums
+//                     through distributed shared memory. For the rest: few
+//                     tokens, where the weights' stream bounds it, and shapes
+//                     with fewer tiles than SMs.
+//
+// Every mbarrier wait is bounded; one that runs out sets the device status
+// word and the block drains its copies and products and exits.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+#include "device_common.cuh"
+#include "gemm_internal.hpp"
+#include "linear_internal.hpp"
+#include "quant_common.cuh"
+
+namespace rns8cuda {
+namespace {
+
+constexpr int BK = 128, UMMA_K = 32, LANES = 128, THREADS = 192;
+constexpr uint32_t SPAN_BYTES = LANES * BK;  // one 128-row operand tile of a stage
+
+struct __align__(64) TcLinear {
+  CUtensorMap tm_tokens, tm_weights;
+  const float *a_scale, *w_scale, *bias;
+  void* out;
+  int64_t m, n, ld_out;
+  uint32_t out_type, total_kb;
+  uint32_t m_tiles, n_tiles, units;  // tokens on lanes
+  uint32_t after_quantize, vector_rows;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ void report_timeout(const TcLinear& p, volatile int* abort_flag) {
+  *abort_flag = 1;
+  atomicOr(p.status, kDevWaitTimeout);
+}
+
+// Blocks until the previous launch on the stream has finished and its writes
+// are visible; returns at once for a launch without that attribute.
+__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Barrier of the four epilogue warps that also ands their predicates.
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster(const void* smem_ptr, uint32_t rank) {
+  uint32_t at;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(smem_ptr)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// ---- channels on lanes -------------------------------------------------------------
+template <int BN, bool GATED>
+struct Lanes {
+  static constexpr int HALVES = GATED ? 2 : 1;
+  static constexpr uint32_t W_BYTES = SPAN_BYTES * HALVES, T_BYTES = BN * BK, STAGE = W_BYTES + T_BYTES;
+  // Two blocks share an SM where the stages are small.
+  static constexpr int STAGES = STAGE <= 24 * 1024 ? 96 * 1024 / STAGE : 196 * 1024 / STAGE;
+  static constexpr uint32_t ACC_COLS = BN * HALVES, TMEM_COLS = ACC_COLS < 32 ? 32 : ACC_COLS;
+  static constexpr size_t SMEM = 1024 + STAGES * STAGE + 256;
+  static_assert(ACC_COLS * LANES * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
+};
+
+template <typename OUT, int BN, bool GATED>
+__global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __grid_constant__ TcLinear p) {
+  using L = Lanes<BN, GATED>;
+  constexpr int STAGES = L::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * L::STAGE);
+  uint64_t* empty = full + STAGES;
+  uint64_t* done = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  uint32_t rank, splits;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x / splits) * LANES, t0 = static_cast<int64_t>(blockIdx.y) * BN;
+  const uint32_t kb0 = p.total_kb * rank / splits, kb1 = p.total_kb * (rank + 1) / splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&p.tm_weights);
+    tma_prefetch_desc(&p.tm_tokens);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, L::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer ----------------
+      auto load_weights = [&](uint32_t stage, uint32_t kb) {
+        uint8_t* at = smem + stage * L::STAGE;
+        mbar_arrive_expect_tx(&full[stage], L::STAGE);
+        tma_load_2d(at, &p.tm_weights, &full[stage], static_cast<int32_t>(kb * BK), static_cast<int32_t>(j0));
+        if (GATED)
+          tma_load_2d(at + SPAN_BYTES, &p.tm_weights, &full[stage], static_cast<int32_t>(kb * BK),
+                      static_cast<int32_t>(p.n + j0));
+      };
+      auto load_tokens = [&](uint32_t stage, uint32_t kb) {
+        tma_load_2d(smem + stage * L::STAGE + L::W_BYTES, &p.tm_tokens, &full[stage], static_cast<int32_t>(kb * BK),
+                    static_cast<int32_t>(t0));
+      };
+      // The first stages' weights do not wait for the tokens to be quantised.
+      const uint32_t early = min(kb1 - kb0, static_cast<uint32_t>(STAGES));
+      for (uint32_t i = 0; i < early; ++i) load_weights(i, kb0 + i);
+      if (p.after_quantize) wait_previous_launch();
+      for (uint32_t i = 0; i < early; ++i) load_tokens(i, kb0 + i);
+      uint32_t pending = (1u << early) - 1, parities = 0, stage = early % STAGES, phase = early / STAGES;
+      for (uint32_t kb = kb0 + early; kb < kb1; ++kb) {
+        if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u)) {
+          if (!*abort_flag) report_timeout(p, abort_flag);
+          break;
+        }
+        load_weights(stage, kb);
+        load_tokens(stage, kb);
+        pending |= 1u << stage;
+        parities = (parities & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      // Every copy has landed before the block may exit.
+      for (int s = 0; s < STAGES; ++s)
+        if (pending & (1u << s)) (void)mbar_wait_bounded(&full[s], (parities >> s) & 1u);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t idesc = make_idesc_i8(LANES, BN, /*b_mn_major=*/false);
+      uint32_t stage = 0, phase = 0;
+      for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        if (*abort_flag || !mbar_wait_bounded(&full[stage], phase)) {
+          if (!*abort_flag) report_timeout(p, abort_flag);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + stage * L::STAGE), st = sw + L::W_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+          const uint64_t tdesc = make_smem_desc_sw128(st + kk * UMMA_K, 16, 1024);
+#pragma unroll
+          for (int h = 0; h < L::HALVES; ++h)
+            tc_mma_i8(tmem_base + h * BN, make_smem_desc_sw128(sw + h * SPAN_BYTES + kk * UMMA_K, 16, 1024), tdesc, idesc,
+                      (kb > kb0 || kk > 0) ? 1u : 0u);
+        }
+        tc_commit(&empty[stage]);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(done);
+      (void)mbar_wait_bounded(done, 0);
+    }
+  } else {
+    // ---------------- epilogue (warps 2..5), first part ----------------
+    if (p.after_quantize) wait_previous_launch();
+    if (!mbar_wait_bounded(done, 0) && !*abort_flag) report_timeout(p, abort_flag);
+    tc_fence_after();
+  }
+
+  const uint32_t quarter = static_cast<uint32_t>(warp & 3), row = quarter * 32 + lane;
+  const int64_t j = j0 + row;
+  const bool channel = warp >= 2 && j < p.n;
+  float ws[L::HALVES] = {}, bias[L::HALVES] = {};
+  if (channel) {
+#pragma unroll
+    for (int h = 0; h < L::HALVES; ++h) {
+      ws[h] = p.w_scale[h * p.n + j];
+      if (p.bias) bias[h] = p.bias[h * p.n + j];
+    }
+  }
+  auto store = [&](int c, int acc0, int acc1) {
+    const int64_t t = t0 + c;
+    if (!channel || t >= p.m) return;
+    const float s = p.a_scale[t];
+    float y = static_cast<float>(acc0) * s * ws[0] + bias[0];
+    if (GATED) y = silu_times(y, static_cast<float>(acc1) * s * ws[L::HALVES - 1] + bias[L::HALVES - 1]);
+    static_cast<OUT*>(p.out)[t * p.ld_out + j] = from_f32<OUT>(y);
+  };
+  int* sums = reinterpret_cast<int*>(smem);  // [ACC_COLS][LANES], once the stages are consumed
+  if (warp >= 2) {
+    const uint32_t taddr = tmem_base + ((quarter * 32u) << 16);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      uint32_t v[L::HALVES][32];
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < L::HALVES; ++h) tmem_ld_32x32b_x32(taddr + (BN < 32 ? 0 : h * BN + c), v[h]);
+#pragma unroll
+      for (int h = 0; h < L::HALVES; ++h) tmem_wait_ld(v[h]);
+      if (BN < 32 && GATED) {  // both halves came with one load
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[L::HALVES - 1][i] = v[0][16 + i];
+      }
+#pragma unroll
+      for (int i = 0; i < (BN < 32 ? BN : 32); ++i) {
+        if (splits == 1) {
+          store(c + i, static_cast<int>(v[0][i]), static_cast<int>(v[L::HALVES - 1][i]));
+        } else {
+#pragma unroll
+          for (int h = 0; h < L::HALVES; ++h) sums[(h * BN + c + i) * LANES + row] = static_cast<int>(v[h][i]);
+        }
+      }
+    }
+  }
+  if (splits > 1) {
+    cluster_sync();
+    if (warp >= 2) {
+      const int c0 = static_cast<int>(BN * rank / splits), c1 = static_cast<int>(BN * (rank + 1) / splits);
+      for (int c = c0; c < c1 && t0 + c < p.m; ++c) {
+        int acc[L::HALVES] = {};
+        for (uint32_t r = 0; r < splits; ++r)
+#pragma unroll
+          for (int h = 0; h < L::HALVES; ++h) acc[h] += ld_cluster(&sums[(h * BN + c) * LANES + row], r);
+        store(c, acc[0], acc[L::HALVES - 1]);
+      }
+    }
+    cluster_sync();  // no block leaves while another reads its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::TMEM_COLS);
+  }
+}
+
+// ---- tokens on lanes ----------------------------------------------------------------
+constexpr int BN = 256, STAGES = 4, GROUP_M = 32;
+constexpr uint32_t STAGE_BYTES = SPAN_BYTES + BN * BK;
+constexpr size_t TOKENS_SMEM = 1024 + STAGES * STAGE_BYTES + 256 + 2 * 2 * BN * sizeof(float);
+
+template <typename OUT, bool GATED>
+__global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_constant__ TcLinear p) {
+  constexpr int COLS = GATED ? BN / 2 : BN;  // output columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* col_scale = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 256);  // [2][BN]
+  float* col_bias = col_scale + 2 * BN;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 128);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&p.tm_weights);
+    tma_prefetch_desc(&p.tm_tokens);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if (p.after_quantize) wait_previous_launch();
+
+  // Tiles run down columns of GROUP_M token tiles, so that the tiles in flight
+  // share operands in L2.
+  auto tile_of = [&](uint32_t u, uint32_t& mt, uint32_t& nt) {
+    const uint32_t span = GROUP_M * p.n_tiles, group = u / span, in = u - group * span;
+    const uint32_t size = min(p.m_tiles - group * GROUP_M, static_cast<uint32_t>(GROUP_M));
+    mt = group * GROUP_M + in % size;
+    nt = in / size;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, pending = 0, parities = 0;
+      bool ok = true;
+      for (uint32_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        uint32_t mt, nt;
+        tile_of(u, mt, nt);
+        const int32_t w0 = static_cast<int32_t>(nt * COLS);
+        const int32_t w1 = GATED ? static_cast<int32_t>(p.n + nt * COLS) : w0 + BN / 2;
+        for (uint32_t kb = 0; kb < p.total_kb; ++kb) {
+          if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u)) {
+            if (!*abort_flag) report_timeout(p, abort_flag);
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[stage], STAGE_BYTES);
+          uint8_t* at = smem + stage * STAGE_BYTES;
+          const int32_t k = static_cast<int32_t>(kb * BK);
+          tma_load_2d(at, &p.tm_tokens, &full[stage], k, static_cast<int32_t>(mt * LANES));
+          tma_load_2d(at + SPAN_BYTES, &p.tm_weights, &full[stage], k, w0);
+          tma_load_2d(at + 2 * SPAN_BYTES, &p.tm_weights, &full[stage], k, w1);
+          pending |= 1u << stage;
+          parities = (parities & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      for (int s = 0; s < STAGES; ++s)
+        if (pending & (1u << s)) (void)mbar_wait_bounded(&full[s], (parities >> s) & 1u);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_i8(LANES, BN, /*b_mn_major=*/false);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (uint32_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        if (*abort_flag || !mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u)) {
+          if (!*abort_flag) report_timeout(p, abort_flag);
+          break;
+        }
+        tc_fence_after();
+        for (uint32_t kb = 0; kb < p.total_kb; ++kb) {
+          if (*abort_flag || !mbar_wait_bounded(&full[stage], phase)) {
+            if (!*abort_flag) report_timeout(p, abort_flag);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES), sb = sa + SPAN_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            tc_mma_i8(tmem_base + acc * BN, make_smem_desc_sw128(sa + kk * UMMA_K, 16, 1024),
+                      make_smem_desc_sw128(sb + kk * UMMA_K, 16, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(&empty[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit(&acc_full[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      tc_commit(drain);
+      (void)mbar_wait_bounded(drain, 0);
+    }
+  } else {
+    // ---------------- epilogue: a thread owns a token ----------------
+    const uint32_t quarter = static_cast<uint32_t>(warp & 3);
+    const int et = threadIdx.x - 64;
+    uint32_t acc = 0, acc_phase = 0;
+    for (uint32_t u = blockIdx.x; u < p.units; u += gridDim.x) {
+      uint32_t mt, nt;
+      tile_of(u, mt, nt);
+      const int64_t n0 = static_cast<int64_t>(nt) * COLS;
+      // The tile's column scales and biases, as laid out in the accumulator.
+      float* cs = col_scale + acc * BN;
+      float* cb = col_bias + acc * BN;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = et + i * 128;
+        const int64_t col = n0 + (GATED ? et : c);
+        const bool in = col < p.n;
+        const int64_t w = GATED ? i * p.n + col : col;
+        cs[c] = in ? p.w_scale[w] : 0.0f;
+        cb[c] = in && p.bias ? p.bias[w] : 0.0f;
+      }
+      const int64_t t = static_cast<int64_t>(mt) * LANES + quarter * 32 + lane;
+      const bool token = t < p.m;
+      const float s = token ? p.a_scale[t] : 0.0f;
+      const bool ok = !*abort_flag && mbar_wait_bounded(&acc_full[acc], acc_phase);
+      if (!ok && !*abort_flag) report_timeout(p, abort_flag);
+      // The column values are in place, and the four warps stop together or
+      // not at all: the next tile's barrier needs all of them.
+      if (!epilogue_all(ok)) break;
+      tc_fence_after();
+      OUT* orow = static_cast<OUT*>(p.out) + t * p.ld_out + n0;
+      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c = 0; c < COLS; c += 32) {
+        uint32_t v[32], up[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + c, v);
+        if (GATED) tmem_ld_32x32b_x32(taddr + BN / 2 + c, up);
+        tmem_wait_ld(v);
+        if (GATED) tmem_wait_ld(up);
+        if (!token || n0 + c >= p.n) continue;
+        __align__(16) OUT o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float y = static_cast<float>(static_cast<int>(v[i])) * s * cs[c + i] + cb[c + i];
+          if (GATED)
+            y = silu_times(y, static_cast<float>(static_cast<int>(up[i])) * s * cs[BN / 2 + c + i] + cb[BN / 2 + c + i]);
+          o[i] = from_f32<OUT>(y);
+        }
+        if (p.vector_rows && n0 + c + 32 <= p.n) {
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(o) / 16); ++i)
+            reinterpret_cast<uint4*>(orow + c)[i] = reinterpret_cast<const uint4*>(o)[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n0 + c + i < p.n) orow[c + i] = o[i];
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&acc_empty[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+// ---- launches --------------------------------------------------------------------------
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, std::atomic<uint64_t>& configured, dim3 grid, unsigned cluster, size_t smem,
+                   const TcLinear& p, cudaStream_t stream) {
+  const cudaError_t e = raise_smem_limit_once(kernel, static_cast<int>(smem), configured);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attrs[2];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attrs;
+  attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+  attrs[cfg.numAttrs].val.clusterDim.x = cluster;
+  attrs[cfg.numAttrs].val.clusterDim.y = 1;
+  attrs[cfg.numAttrs].val.clusterDim.z = 1;
+  ++cfg.numAttrs;
+  if (p.after_quantize) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename OUT, int N, bool GATED>
+cudaError_t launch_channels(const TcLinear& p, dim3 grid, unsigned splits, cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  return launch(linear_channels_kernel<OUT, N, GATED>, configured, grid, splits, Lanes<N, GATED>::SMEM, p, stream);
+}
+template <typename OUT, bool GATED>
+cudaError_t launch_tokens(const TcLinear& p, unsigned grid, cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  return launch(linear_tokens_kernel<OUT, GATED>, configured, dim3(grid), 1, TOKENS_SMEM, p, stream);
+}
+
+template <typename F>
+cudaError_t with_type(uint32_t type, F&& f) {
+  if (type == RNS8_CUDA_TYPE_BF16) return f(__nv_bfloat16{});
+  if (type == RNS8_CUDA_TYPE_F16) return f(__half{});
+  return f(float{});
+}
+
+}  // namespace
+
+cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
+  TcLinear p{};
+  p.a_scale = a.a_scale, p.w_scale = a.w_scale, p.bias = a.bias, p.out = a.out;
+  p.m = a.m, p.n = a.n, p.ld_out = a.ld_out, p.out_type = a.out_type;
+  p.total_kb = static_cast<uint32_t>((a.k + BK - 1) / BK);
+  p.after_quantize = a.after_quantize;
+  p.status = a.status;
+  const size_t elem = a.out_type == RNS8_CUDA_TYPE_F32 ? 4 : 2;
+  p.vector_rows = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ld_out * elem % 16 == 0;
+  const int64_t w_rows = a.gated ? 2 * a.n : a.n;
+  if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, LANES)) return cudaErrorInvalidValue;
+
+  const int cols = a.gated ? BN / 2 : BN;
+  const uint64_t m_tiles = (a.m + LANES - 1) / LANES, n_tiles = (a.n + cols - 1) / cols;
+  if (m_tiles * n_tiles >= static_cast<uint64_t>(sm_count) * 3 / 4) {
+    if (m_tiles * n_tiles >= (1ull << 32)) return cudaErrorInvalidValue;
+    if (!encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, LANES)) return cudaErrorInvalidValue;
+    p.m_tiles = static_cast<uint32_t>(m_tiles);
+    p.n_tiles = static_cast<uint32_t>(n_tiles);
+    p.units = p.m_tiles * p.n_tiles;
+    const unsigned grid = std::min<unsigned>(p.units, static_cast<unsigned>(sm_count));
+    return with_type(a.out_type, [&](auto t) {
+      using OUT = decltype(t);
+      return a.gated ? launch_tokens<OUT, true>(p, grid, stream) : launch_tokens<OUT, false>(p, grid, stream);
+    });
+  }
+
+  const int most = a.gated ? 128 : 256;
+  int tile = 16;
+  while (tile < most && tile < a.m) tile *= 2;
+  if (!encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, static_cast<uint32_t>(tile))) return cudaErrorInvalidValue;
+  const uint64_t token_tiles = (a.m + tile - 1) / tile, channel_tiles = (a.n + LANES - 1) / LANES;
+  const uint64_t tiles = token_tiles * channel_tiles;
+  unsigned splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= static_cast<uint64_t>(sm_count) * 5 / 4 && p.total_kb >= 4 * splits) splits *= 2;
+  const dim3 grid(static_cast<unsigned>(channel_tiles * splits), static_cast<unsigned>(token_tiles));
+  return with_type(a.out_type, [&](auto t) {
+    using OUT = decltype(t);
+    auto go = [&](auto g) {
+      constexpr bool G = decltype(g)::value;
+      switch (tile) {
+        case 16: return launch_channels<OUT, 16, G>(p, grid, splits, stream);
+        case 32: return launch_channels<OUT, 32, G>(p, grid, splits, stream);
+        case 64: return launch_channels<OUT, 64, G>(p, grid, splits, stream);
+        case 128: return launch_channels<OUT, 128, G>(p, grid, splits, stream);
+        default: return launch_channels<OUT, G ? 128 : 256, G>(p, grid, splits, stream);
+      }
+    };
+    return a.gated ? go(std::true_type{}) : go(std::false_type{});
+  });
+}
+
+}  // namespace rns8cuda
