@@ -1,5 +1,7 @@
 // C entry points of the 8-bit operators (include/rns8/rns8_quant.h): argument
 // checks, then the launch on the caller's device and stream.
+#include <atomic>
+
 #include "api_internal.hpp"
 #include "quant_kernels.hpp"
 
@@ -23,12 +25,17 @@ bool valid_rows(const void* p, int64_t rows, int64_t cols, int64_t ld, uint32_t 
   return p && aligned_to(p, elem) && ld >= cols && ld <= kMaxElements / (rows > 0 ? rows : 1);
 }
 
+// Multiprocessors of a device, asked once per device.
 int sm_count_of(int device_id) {
-  int count = 0;
+  static std::atomic<int> known[64];
+  const bool slot = device_id >= 0 && device_id < 64;
+  int count = slot ? known[device_id].load(std::memory_order_relaxed) : 0;
+  if (count > 0) return count;
   if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device_id) != cudaSuccess || count <= 0) {
     (void)cudaGetLastError();
     return 148;
   }
+  if (slot) known[device_id].store(count, std::memory_order_relaxed);
   return count;
 }
 
@@ -99,7 +106,7 @@ extern "C" rns8_status rns8_cuda_quantize_rows_device(const rns8_cuda_quantize_d
 
 extern "C" uint64_t rns8_cuda_linear_scratch_bytes(const rns8_cuda_linear_desc* desc) {
   if (check_linear(desc) != RNS8_SUCCESS || desc->m == 0) return 0;
-  return rns8cuda::linear_scratch_bytes(*desc, sm_count_of(desc->device_id));
+  return rns8cuda::linear_scratch_bytes(*desc);
 }
 
 extern "C" rns8_status rns8_cuda_linear_device(const rns8_cuda_linear_desc* desc) {
@@ -109,10 +116,9 @@ extern "C" rns8_status rns8_cuda_linear_device(const rns8_cuda_linear_desc* desc
   if (desc->m == 0) return RNS8_SUCCESS;
   rns8host::DeviceScope scope(desc->device_id);
   if (!scope.ok) return RNS8_BACKEND_FAILURE;
-  const int sms = sm_count_of(desc->device_id);
-  const uint64_t need = rns8cuda::linear_scratch_bytes(*desc, sms);
+  const uint64_t need = rns8cuda::linear_scratch_bytes(*desc);
   if (need && (!desc->scratch || desc->scratch_bytes < need)) return RNS8_WORKSPACE_TOO_SMALL;
-  return launch_result(rns8cuda::linear(*desc, sms, static_cast<cudaStream_t>(desc->stream)));
+  return launch_result(rns8cuda::linear(*desc, sm_count_of(desc->device_id), static_cast<cudaStream_t>(desc->stream)));
 }
 
 extern "C" rns8_status rns8_cuda_residual_norm_device(const rns8_cuda_residual_norm_desc* desc) {

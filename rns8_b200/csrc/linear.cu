@@ -5,6 +5,7 @@
 #include "linear_internal.hpp"
 #include "quant_common.cuh"
 #include "quant_kernels.hpp"
+#include "quant_launch.cuh"
 
 namespace rns8cuda {
 namespace {
@@ -16,6 +17,8 @@ bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p
 // cols are zero.
 __global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ src, int64_t rows, int64_t cols,
                                                          int64_t ld, int8_t* __restrict__ dst, int64_t ld_dst) {
+  wait_previous_launch();
+  allow_next_launch();
   const int64_t per_row = ld_dst / 16, total = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -32,30 +35,23 @@ cudaError_t align_rows(const int8_t* src, int64_t rows, int64_t cols, int64_t ld
                        int sm_count, cudaStream_t stream) {
   const int64_t chunks = rows * (ld_dst / 16);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((chunks + 255) / 256, sm_count * 16));
-  align_rows_kernel<<<grid, 256, 0, stream>>>(src, rows, cols, ld, dst, ld_dst);
-  return cudaGetLastError();
+  return launch_chained(align_rows_kernel, dim3(grid), 256, 0, 1, stream, src, rows, cols, ld, dst, ld_dst);
 }
 
-// What a call needs around its product kernel, and where in scratch.
+// What a call needs before its product, and where in scratch.
 struct Steps {
-  LinearArgs args;
-  bool align_w, align_a, quantize, gemv;
-  int64_t ld;
-  uint64_t at_w, at_a, at_scale, bytes;
+  bool align_w, align_a, quantize;
+  int64_t w_rows, ld;
+  uint64_t at_a, at_scale, bytes;
 };
 Steps plan(const rns8_cuda_linear_desc& d) {
   Steps s{};
-  s.args = LinearArgs{d.a,      d.w,      d.a_scale,  d.w_scale, d.bias, d.out, d.m, d.n, d.k, d.ld_a, d.ld_w, d.ld_out,
-                      d.a_type, d.out_type, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, false, d.status};
-  const int64_t w_rows = s.args.gated ? 2 * d.n : d.n;
+  s.w_rows = (d.flags & RNS8_CUDA_LINEAR_GATED) ? 2 * d.n : d.n;
   s.ld = static_cast<int64_t>(round_up(d.k, 16));
   s.align_w = !aligned16(d.w, d.ld_w);
-  LinearArgs aligned = s.args;
-  if (s.align_w) aligned.w = nullptr, aligned.ld_w = s.ld;
-  s.gemv = gemv_supported(aligned);
-  s.quantize = !s.gemv && d.a_type != RNS8_CUDA_TYPE_I8;
-  s.align_a = !s.gemv && !s.quantize && !aligned16(d.a, d.ld_a);
-  if (s.align_w) s.bytes = round_up(static_cast<uint64_t>(w_rows) * s.ld, 256);
+  s.quantize = d.a_type != RNS8_CUDA_TYPE_I8;
+  s.align_a = !s.quantize && !aligned16(d.a, d.ld_a);
+  if (s.align_w) s.bytes = round_up(static_cast<uint64_t>(s.w_rows) * s.ld, 256);
   s.at_a = s.bytes;
   if (s.quantize || s.align_a) s.bytes += round_up(static_cast<uint64_t>(d.m) * s.ld, 256);
   s.at_scale = s.bytes;
@@ -66,34 +62,33 @@ Steps plan(const rns8_cuda_linear_desc& d) {
 
 }  // namespace
 
-uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d, int) { return plan(d).bytes; }
+uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d) { return plan(d).bytes; }
 
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream) {
-  Steps s = plan(d);
-  LinearArgs& p = s.args;
+  const Steps s = plan(d);
+  LinearArgs p{static_cast<const int8_t*>(d.a), d.w, d.a_scale, d.w_scale, d.bias, d.out, d.m, d.n, d.k, d.ld_a, d.ld_w,
+               d.ld_out, d.out_type, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, s.quantize, d.status};
   int8_t* scratch = reinterpret_cast<int8_t*>(round_up(reinterpret_cast<uintptr_t>(d.scratch), 256));
   cudaError_t e = cudaSuccess;
   if (s.align_w) {
-    e = align_rows(d.w, p.gated ? 2 * d.n : d.n, d.k, d.ld_w, scratch, s.ld, sm_count, stream);
+    e = align_rows(d.w, s.w_rows, d.k, d.ld_w, scratch, s.ld, sm_count, stream);
     if (e != cudaSuccess) return e;
     p.w = scratch;
     p.ld_w = s.ld;
   }
-  if (s.gemv) return linear_gemv(p, sm_count, stream);
-  if (s.align_a) {
-    e = align_rows(static_cast<const int8_t*>(d.a), d.m, d.k, d.ld_a, scratch + s.at_a, s.ld, sm_count, stream);
-    p.a = scratch + s.at_a;
-    p.ld_a = s.ld;
-  } else if (s.quantize) {
+  if (s.align_a || s.quantize) {
+    int8_t* q = scratch + s.at_a;
     float* scale = reinterpret_cast<float*>(scratch + s.at_scale);
-    e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, scratch + s.at_a, s.ld, scale, stream);
-    p.a = scratch + s.at_a;
+    if (s.quantize) {
+      e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, q, s.ld, scale, stream);
+      p.a_scale = scale;
+    } else {
+      e = align_rows(p.a, d.m, d.k, d.ld_a, q, s.ld, sm_count, stream);
+    }
+    if (e != cudaSuccess) return e;
+    p.a = q;
     p.ld_a = s.ld;
-    p.a_type = RNS8_CUDA_TYPE_I8;
-    p.a_scale = scale;
-    p.after_quantize = true;
   }
-  if (e != cudaSuccess) return e;
   return linear_tc(p, sm_count, stream);
 }
 

@@ -9,12 +9,12 @@
 //                     per tile, two accumulators, so that a tile's epilogue
 //                     runs under the next tile's products. For products with
 //                     about a tile per SM or more.
-//   channels on lanes One tile of 128 output channels (gated: 128 gate and 128
-//                     up rows) x 16..256 tokens per cluster; the blocks of a
-//                     cluster split k and join their exact integer sums
-//                     through distributed shared memory. For the rest: few
-//                     tokens, where the weights' stream bounds it, and shapes
-//                     with fewer tiles than SMs.
+//   channels on lanes One tile of 128 weight rows (gated: 64 gate rows and
+//                     their 64 up rows) x 16..256 tokens per cluster; the
+//                     blocks of a cluster split k and join their exact integer
+//                     sums through distributed shared memory. For the rest:
+//                     few tokens, where the weights' stream bounds it, and
+//                     shapes with fewer tiles than SMs.
 //
 // Every mbarrier wait is bounded; one that runs out sets the device status
 // word and the block drains its copies and products and exits.
@@ -28,11 +28,13 @@
 #include "gemm_internal.hpp"
 #include "linear_internal.hpp"
 #include "quant_common.cuh"
+#include "quant_launch.cuh"
 
 namespace rns8cuda {
 namespace {
 
 constexpr int BK = 128, UMMA_K = 32, LANES = 128, THREADS = 192;
+constexpr int kMaxSplits = 8;  // blocks of a cluster
 constexpr uint32_t SPAN_BYTES = LANES * BK;  // one 128-row operand tile of a stage
 
 struct __align__(64) TcLinear {
@@ -40,7 +42,7 @@ struct __align__(64) TcLinear {
   const float *a_scale, *w_scale, *bias;
   void* out;
   int64_t m, n, ld_out;
-  uint32_t out_type, total_kb;
+  uint32_t total_kb;
   uint32_t m_tiles, n_tiles, units;  // tokens on lanes
   uint32_t after_quantize, vector_rows;
   uint32_t* status;
@@ -50,10 +52,6 @@ __device__ __forceinline__ void report_timeout(const TcLinear& p, volatile int* 
   *abort_flag = 1;
   atomicOr(p.status, kDevWaitTimeout);
 }
-
-// Blocks until the previous launch on the stream has finished and its writes
-// are visible; returns at once for a launch without that attribute.
-__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
@@ -75,30 +73,68 @@ __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ int ld_cluster(const void* smem_ptr, uint32_t rank) {
+// Sixteen bytes of block `rank`'s shared memory.
+__device__ __forceinline__ int4 ld_cluster(const void* smem_ptr, uint32_t rank) {
   uint32_t at;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(smem_ptr)), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  int4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(smem_ptr)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at));
   return v;
 }
 
+// Stores G tokens x 32 channels of a warp: lane l holds channel j0 + l of every
+// token, the warp's slice of shared memory turns that into runs of 32 channels
+// and each lane stores G consecutive channels of token l / (32 / G) as one
+// word (a store of single elements a token costs some 50 cycles each).
+// `wide`: whole words are aligned. Tokens from `tokens` on and channels from
+// `channels` on are left out.
+template <typename OUT, int G>
+__device__ __forceinline__ void store_turned(OUT* __restrict__ out, int64_t ld, const float (&y)[G], OUT* slice,
+                                             int lane, int tokens, int64_t channels, bool wide) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < G; ++i) slice[i * 32 + lane] = from_f32<OUT>(y[i]);
+  __syncwarp();
+  constexpr int LANES_PER_TOKEN = 32 / G;
+  const int t = lane / LANES_PER_TOKEN, c = lane % LANES_PER_TOKEN * G;
+  if (t >= tokens) return;
+  OUT* to = out + t * ld + c;
+  const OUT* from = slice + t * 32 + c;
+  if (wide && c + G <= channels) {
+    if constexpr (G * sizeof(OUT) == 8) {
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(G * sizeof(OUT) / 16); ++i)
+        reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      if (c + i < channels) to[i] = from[i];
+  }
+}
+
 // ---- channels on lanes -------------------------------------------------------------
-template <int BN, bool GATED>
+template <int BN>
 struct Lanes {
-  static constexpr int HALVES = GATED ? 2 : 1;
-  static constexpr uint32_t W_BYTES = SPAN_BYTES * HALVES, T_BYTES = BN * BK, STAGE = W_BYTES + T_BYTES;
-  // Two blocks share an SM where the stages are small.
-  static constexpr int STAGES = STAGE <= 24 * 1024 ? 96 * 1024 / STAGE : 196 * 1024 / STAGE;
-  static constexpr uint32_t ACC_COLS = BN * HALVES, TMEM_COLS = ACC_COLS < 32 ? 32 : ACC_COLS;
-  static constexpr size_t SMEM = 1024 + STAGES * STAGE + 256;
-  static_assert(ACC_COLS * LANES * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
+  static constexpr uint32_t STAGE = SPAN_BYTES + BN * BK;
+  // Two blocks share an SM (one for 256 tokens): a block alone streams at no
+  // more than half of an SM's share of HBM.
+  static constexpr int PER_SM = BN <= 128 ? 2 : 1;
+  static constexpr int STAGES = (PER_SM == 2 ? 104 * 1024 : 196 * 1024) / STAGE;
+  static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
+  static constexpr uint32_t TURN = 8 * 32 * 4;  // store_turned's slice of a warp
+  static constexpr size_t SMEM = 1024 + STAGES * STAGE + 256 + BN * sizeof(float) + 4 * TURN;
+  static_assert(BN * LANES * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
 };
 
 template <typename OUT, int BN, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __grid_constant__ TcLinear p) {
-  using L = Lanes<BN, GATED>;
-  constexpr int STAGES = L::STAGES;
+  using L = Lanes<BN>;
+  constexpr int STAGES = L::STAGES, CHANNELS = GATED ? LANES / 2 : LANES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * L::STAGE);
@@ -106,12 +142,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   uint64_t* done = empty + STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* token_scale = reinterpret_cast<float*>(smem + STAGES * L::STAGE + 256);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   uint32_t rank, splits;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x / splits) * LANES, t0 = static_cast<int64_t>(blockIdx.y) * BN;
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x / splits) * CHANNELS, t0 = static_cast<int64_t>(blockIdx.y) * BN;
   const uint32_t kb0 = p.total_kb * rank / splits, kb1 = p.total_kb * (rank + 1) / splits;
 
   if (threadIdx.x == 0) {
@@ -133,6 +170,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // After this call's own quantisation the weights are not waited for: that
+  // kernel has seen everything before it complete.
+  if (!p.after_quantize) wait_previous_launch();
+  allow_next_launch();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -142,11 +183,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
         mbar_arrive_expect_tx(&full[stage], L::STAGE);
         tma_load_2d(at, &p.tm_weights, &full[stage], static_cast<int32_t>(kb * BK), static_cast<int32_t>(j0));
         if (GATED)
-          tma_load_2d(at + SPAN_BYTES, &p.tm_weights, &full[stage], static_cast<int32_t>(kb * BK),
+          tma_load_2d(at + SPAN_BYTES / 2, &p.tm_weights, &full[stage], static_cast<int32_t>(kb * BK),
                       static_cast<int32_t>(p.n + j0));
       };
       auto load_tokens = [&](uint32_t stage, uint32_t kb) {
-        tma_load_2d(smem + stage * L::STAGE + L::W_BYTES, &p.tm_tokens, &full[stage], static_cast<int32_t>(kb * BK),
+        tma_load_2d(smem + stage * L::STAGE + SPAN_BYTES, &p.tm_tokens, &full[stage], static_cast<int32_t>(kb * BK),
                     static_cast<int32_t>(t0));
       };
       // The first stages' weights do not wait for the tokens to be quantised.
@@ -184,15 +225,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
           break;
         }
         tc_fence_after();
-        const uint32_t sw = smem_u32(smem + stage * L::STAGE), st = sw + L::W_BYTES;
+        const uint32_t sw = smem_u32(smem + stage * L::STAGE), st = sw + SPAN_BYTES;
 #pragma unroll
-        for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-          const uint64_t tdesc = make_smem_desc_sw128(st + kk * UMMA_K, 16, 1024);
-#pragma unroll
-          for (int h = 0; h < L::HALVES; ++h)
-            tc_mma_i8(tmem_base + h * BN, make_smem_desc_sw128(sw + h * SPAN_BYTES + kk * UMMA_K, 16, 1024), tdesc, idesc,
-                      (kb > kb0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < BK / UMMA_K; ++kk)
+          tc_mma_i8(tmem_base, make_smem_desc_sw128(sw + kk * UMMA_K, 16, 1024),
+                    make_smem_desc_sw128(st + kk * UMMA_K, 16, 1024), idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
         if (++stage == STAGES) {
           stage = 0;
@@ -205,65 +242,90 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   } else {
     // ---------------- epilogue (warps 2..5), first part ----------------
     if (p.after_quantize) wait_previous_launch();
-    if (!mbar_wait_bounded(done, 0) && !*abort_flag) report_timeout(p, abort_flag);
-    tc_fence_after();
+    for (int c = threadIdx.x - 64; c < BN; c += 128) token_scale[c] = t0 + c < p.m ? p.a_scale[t0 + c] : 0.0f;
   }
 
-  const uint32_t quarter = static_cast<uint32_t>(warp & 3), row = quarter * 32 + lane;
-  const int64_t j = j0 + row;
-  const bool channel = warp >= 2 && j < p.n;
-  float ws[L::HALVES] = {}, bias[L::HALVES] = {};
-  if (channel) {
-#pragma unroll
-    for (int h = 0; h < L::HALVES; ++h) {
-      ws[h] = p.w_scale[h * p.n + j];
-      if (p.bias) bias[h] = p.bias[h * p.n + j];
+  // A thread of the epilogue owns a channel: in the direct form (an ungated
+  // tile of one block) its accumulator lane, else a lane of the joined sums,
+  // where a gated tile has half as many and splits the tokens over its warps.
+  const int ew = warp & 3, cw = GATED ? ew & 1 : ew;
+  const int64_t w0 = j0 + cw * 32, j = w0 + lane;  // the warp's first channel, this thread's
+  const int tokens = static_cast<int>(min(p.m - t0, static_cast<int64_t>(BN)));
+  OUT* out = static_cast<OUT*>(p.out) + t0 * p.ld_out + w0;
+  OUT* slice = reinterpret_cast<OUT*>(reinterpret_cast<uint8_t*>(token_scale + BN) + ew * L::TURN);
+  float ws = 0.0f, bias = 0.0f, up_ws = 0.0f, up_bias = 0.0f;
+  if (warp >= 2 && j < p.n) {
+    ws = p.w_scale[j];
+    if (p.bias) bias = p.bias[j];
+    if (GATED) {
+      up_ws = p.w_scale[p.n + j];
+      if (p.bias) up_bias = p.bias[p.n + j];
     }
   }
-  auto store = [&](int c, int acc0, int acc1) {
-    const int64_t t = t0 + c;
-    if (!channel || t >= p.m) return;
-    const float s = p.a_scale[t];
-    float y = static_cast<float>(acc0) * s * ws[0] + bias[0];
-    if (GATED) y = silu_times(y, static_cast<float>(acc1) * s * ws[L::HALVES - 1] + bias[L::HALVES - 1]);
-    static_cast<OUT*>(p.out)[t * p.ld_out + j] = from_f32<OUT>(y);
+  auto value = [&](int c, int acc, int up) {
+    const float s = token_scale[c];
+    const float y = static_cast<float>(acc) * s * ws + bias;
+    return GATED ? silu_times(y, static_cast<float>(up) * s * up_ws + up_bias) : y;
   };
-  int* sums = reinterpret_cast<int*>(smem);  // [ACC_COLS][LANES], once the stages are consumed
+  const bool direct = !GATED && splits == 1;
+  int4* sums = reinterpret_cast<int4*>(smem);  // [BN / 4][LANES], once the stages are consumed
   if (warp >= 2) {
-    const uint32_t taddr = tmem_base + ((quarter * 32u) << 16);
+    if (!mbar_wait_bounded(done, 0) && !*abort_flag) report_timeout(p, abort_flag);
+    (void)epilogue_all(true);  // the token scales are in place
+    tc_fence_after();
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
-      uint32_t v[L::HALVES][32];
+    for (int c = 0; c < tokens; c += 32) {
+      uint32_t v[32];
       __syncwarp();
+      tmem_ld_32x32b_x32(taddr + c, v);
+      tmem_wait_ld(v);
 #pragma unroll
-      for (int h = 0; h < L::HALVES; ++h) tmem_ld_32x32b_x32(taddr + (BN < 32 ? 0 : h * BN + c), v[h]);
+      for (int i = 0; i < (BN < 32 ? BN : 32); i += 8) {
+        if (direct) {
+          float y[8];
 #pragma unroll
-      for (int h = 0; h < L::HALVES; ++h) tmem_wait_ld(v[h]);
-      if (BN < 32 && GATED) {  // both halves came with one load
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[L::HALVES - 1][i] = v[0][16 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < (BN < 32 ? BN : 32); ++i) {
-        if (splits == 1) {
-          store(c + i, static_cast<int>(v[0][i]), static_cast<int>(v[L::HALVES - 1][i]));
+          for (int e = 0; e < 8; ++e) y[e] = value(c + i + e, static_cast<int>(v[i + e]), 0);
+          store_turned<OUT, 8>(out + (c + i) * p.ld_out, p.ld_out, y, slice, lane, tokens - c - i, p.n - w0,
+                               p.vector_rows);
         } else {
 #pragma unroll
-          for (int h = 0; h < L::HALVES; ++h) sums[(h * BN + c + i) * LANES + row] = static_cast<int>(v[h][i]);
+          for (int e = i; e < i + 8; e += 4)
+            sums[((c + e) / 4) * LANES + ew * 32 + lane] =
+                make_int4(static_cast<int>(v[e]), static_cast<int>(v[e + 1]), static_cast<int>(v[e + 2]),
+                          static_cast<int>(v[e + 3]));
         }
       }
     }
   }
-  if (splits > 1) {
+  if (!direct) {
+    // Each block of the cluster joins a share of the tile's tokens, four at a
+    // time; all the blocks' parts of them are in flight together.
     cluster_sync();
     if (warp >= 2) {
-      const int c0 = static_cast<int>(BN * rank / splits), c1 = static_cast<int>(BN * (rank + 1) / splits);
-      for (int c = c0; c < c1 && t0 + c < p.m; ++c) {
-        int acc[L::HALVES] = {};
-        for (uint32_t r = 0; r < splits; ++r)
+      constexpr int WARPS_PER_TOKEN = CHANNELS / 32, SHARES = 4 / WARPS_PER_TOKEN;
+      const int step = 4 * static_cast<int>(splits) * SHARES;
+      for (int c = 4 * (static_cast<int>(rank) * SHARES + ew / WARPS_PER_TOKEN); c < tokens; c += step) {
+        int4 part[GATED ? 2 : 1][kMaxSplits];
 #pragma unroll
-          for (int h = 0; h < L::HALVES; ++h) acc[h] += ld_cluster(&sums[(h * BN + c) * LANES + row], r);
-        store(c, acc[0], acc[L::HALVES - 1]);
+        for (int r = 0; r < kMaxSplits; ++r)
+#pragma unroll
+          for (int h = 0; h < (GATED ? 2 : 1); ++h)
+            part[h][r] = r < static_cast<int>(splits)
+                             ? ld_cluster(&sums[(c / 4) * LANES + h * CHANNELS + cw * 32 + lane], r)
+                             : make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h)
+#pragma unroll
+          for (int r = 1; r < kMaxSplits; ++r) {
+            part[h][0].x += part[h][r].x;
+            part[h][0].y += part[h][r].y;
+            part[h][0].z += part[h][r].z;
+            part[h][0].w += part[h][r].w;
+          }
+        const int4 a = part[0][0], u = part[GATED ? 1 : 0][0];
+        const float y[4] = {value(c, a.x, u.x), value(c + 1, a.y, u.y), value(c + 2, a.z, u.z), value(c + 3, a.w, u.w)};
+        store_turned<OUT, 4>(out + c * p.ld_out, p.ld_out, y, slice, lane, tokens - c, p.n - w0, p.vector_rows);
       }
     }
     cluster_sync();  // no block leaves while another reads its sums
@@ -319,7 +381,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if (p.after_quantize) wait_previous_launch();
+  wait_previous_launch();
+  allow_next_launch();
 
   // Tiles run down columns of GROUP_M token tiles, so that the tiles in flight
   // share operands in L2.
@@ -481,30 +544,13 @@ cudaError_t launch(Kernel kernel, std::atomic<uint64_t>& configured, dim3 grid, 
                    const TcLinear& p, cudaStream_t stream) {
   const cudaError_t e = raise_smem_limit_once(kernel, static_cast<int>(smem), configured);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attrs[2];
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attrs;
-  attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-  attrs[cfg.numAttrs].val.clusterDim.x = cluster;
-  attrs[cfg.numAttrs].val.clusterDim.y = 1;
-  attrs[cfg.numAttrs].val.clusterDim.z = 1;
-  ++cfg.numAttrs;
-  if (p.after_quantize) {
-    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return launch_chained(kernel, grid, THREADS, smem, cluster, stream, p);
 }
 
 template <typename OUT, int N, bool GATED>
 cudaError_t launch_channels(const TcLinear& p, dim3 grid, unsigned splits, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  return launch(linear_channels_kernel<OUT, N, GATED>, configured, grid, splits, Lanes<N, GATED>::SMEM, p, stream);
+  return launch(linear_channels_kernel<OUT, N, GATED>, configured, grid, splits, Lanes<N>::SMEM, p, stream);
 }
 template <typename OUT, bool GATED>
 cudaError_t launch_tokens(const TcLinear& p, unsigned grid, cudaStream_t stream) {
@@ -524,20 +570,20 @@ cudaError_t with_type(uint32_t type, F&& f) {
 cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
   TcLinear p{};
   p.a_scale = a.a_scale, p.w_scale = a.w_scale, p.bias = a.bias, p.out = a.out;
-  p.m = a.m, p.n = a.n, p.ld_out = a.ld_out, p.out_type = a.out_type;
+  p.m = a.m, p.n = a.n, p.ld_out = a.ld_out;
   p.total_kb = static_cast<uint32_t>((a.k + BK - 1) / BK);
   p.after_quantize = a.after_quantize;
   p.status = a.status;
   const size_t elem = a.out_type == RNS8_CUDA_TYPE_F32 ? 4 : 2;
   p.vector_rows = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ld_out * elem % 16 == 0;
   const int64_t w_rows = a.gated ? 2 * a.n : a.n;
-  if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, LANES)) return cudaErrorInvalidValue;
-
   const int cols = a.gated ? BN / 2 : BN;
   const uint64_t m_tiles = (a.m + LANES - 1) / LANES, n_tiles = (a.n + cols - 1) / cols;
   if (m_tiles * n_tiles >= static_cast<uint64_t>(sm_count) * 3 / 4) {
     if (m_tiles * n_tiles >= (1ull << 32)) return cudaErrorInvalidValue;
-    if (!encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, LANES)) return cudaErrorInvalidValue;
+    if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, LANES) ||
+        !encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, LANES))
+      return cudaErrorInvalidValue;
     p.m_tiles = static_cast<uint32_t>(m_tiles);
     p.n_tiles = static_cast<uint32_t>(n_tiles);
     p.units = p.m_tiles * p.n_tiles;
@@ -548,14 +594,16 @@ cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
     });
   }
 
-  const int most = a.gated ? 128 : 256;
   int tile = 16;
-  while (tile < most && tile < a.m) tile *= 2;
-  if (!encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, static_cast<uint32_t>(tile))) return cudaErrorInvalidValue;
-  const uint64_t token_tiles = (a.m + tile - 1) / tile, channel_tiles = (a.n + LANES - 1) / LANES;
-  const uint64_t tiles = token_tiles * channel_tiles;
+  while (tile < 256 && tile < a.m) tile *= 2;
+  const int channels = a.gated ? LANES / 2 : LANES;
+  if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, static_cast<uint32_t>(channels)) ||
+      !encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, static_cast<uint32_t>(tile)))
+    return cudaErrorInvalidValue;
+  const uint64_t token_tiles = (a.m + tile - 1) / tile, channel_tiles = (a.n + channels - 1) / channels;
+  const uint64_t tiles = token_tiles * channel_tiles, room = static_cast<uint64_t>(sm_count) * (tile <= 128 ? 2 : 1);
   unsigned splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= static_cast<uint64_t>(sm_count) * 5 / 4 && p.total_kb >= 4 * splits) splits *= 2;
+  while (splits < kMaxSplits && tiles * splits * 2 <= room && p.total_kb >= 4 * splits) splits *= 2;
   const dim3 grid(static_cast<unsigned>(channel_tiles * splits), static_cast<unsigned>(token_tiles));
   return with_type(a.out_type, [&](auto t) {
     using OUT = decltype(t);
@@ -566,7 +614,7 @@ cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
         case 32: return launch_channels<OUT, 32, G>(p, grid, splits, stream);
         case 64: return launch_channels<OUT, 64, G>(p, grid, splits, stream);
         case 128: return launch_channels<OUT, 128, G>(p, grid, splits, stream);
-        default: return launch_channels<OUT, G ? 128 : 256, G>(p, grid, splits, stream);
+        default: return launch_channels<OUT, 256, G>(p, grid, splits, stream);
       }
     };
     return a.gated ? go(std::true_type{}) : go(std::false_type{});

@@ -36,6 +36,15 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// Vectors of 8 a thread of a row kernel holds. Few rows are a matter of latency:
+// one vector a thread. With rows for every SM, blocks of at most 256 threads
+// let the loads of one row run under the reductions of the others.
+inline int row_vectors(int64_t rows, int vecs) {
+  if (vecs > 1024) return 4;
+  if (rows < 256 || vecs <= 256) return 1;
+  return vecs <= 512 ? 2 : 4;
+}
+
 // Index of element (v, e) of this thread's part of a row.
 template <bool ALIGNED>
 __device__ __forceinline__ int row_index(int v, int e, int threads, int tid) {

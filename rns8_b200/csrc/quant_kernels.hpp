@@ -13,7 +13,7 @@ namespace rns8cuda {
 cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q,
                           int64_t ld_q, float* scale, cudaStream_t stream);
 
-uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d, int sm_count);
+uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d);
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream);
 
 cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t stream);

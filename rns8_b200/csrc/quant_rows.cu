@@ -4,6 +4,7 @@
 
 #include "quant_common.cuh"
 #include "quant_kernels.hpp"
+#include "quant_launch.cuh"
 
 namespace rns8cuda {
 namespace {
@@ -13,6 +14,8 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict
                                                              int8_t* __restrict__ q, int64_t ld_q,
                                                              float* __restrict__ scale) {
   __shared__ uint32_t slots[32];
+  wait_previous_launch();
+  allow_next_launch();
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ld_x;
   float v[NV][8];
@@ -34,6 +37,8 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* __res
                                                                   int8_t* __restrict__ q, int64_t ld_q,
                                                                   float* __restrict__ scale) {
   __shared__ uint32_t slots[32];
+  wait_previous_launch();
+  allow_next_launch();
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ld_x;
   uint32_t top = 0;
@@ -49,29 +54,23 @@ cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int8_t*
                    cudaStream_t stream) {
   const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(q) % 8 == 0 && ld_q % 8 == 0;
-  const unsigned grid = static_cast<unsigned>(rows);
-  if (cols > 1024 * 8 * 4) {
-    quantize_long_rows_kernel<T><<<grid, 1024, 0, stream>>>(x, cols, ld_x, q, ld_q, scale);
-    return cudaGetLastError();
-  }
-  const int c = static_cast<int>(cols);
-  const int vecs = (c + 7) / 8;
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (cols > 1024 * 8 * 4)
+    return launch_chained(quantize_long_rows_kernel<T>, grid, 1024, 0, 1, stream, x, cols, ld_x, q, ld_q, scale);
+  const int c = static_cast<int>(cols), vecs = (c + 7) / 8;
   auto go = [&](auto nv, auto al) {
     constexpr int NV = decltype(nv)::value;
-    const int threads = std::max(32, ((vecs + NV - 1) / NV + 31) / 32 * 32);
-    quantize_rows_kernel<T, decltype(al)::value, NV><<<grid, threads, 0, stream>>>(x, c, ld_x, q, ld_q, scale);
+    const unsigned threads = static_cast<unsigned>(std::max(32, ((vecs + NV - 1) / NV + 31) / 32 * 32));
+    return launch_chained(quantize_rows_kernel<T, decltype(al)::value, NV>, grid, threads, 0, 1, stream, x, c, ld_x, q,
+                          ld_q, scale);
   };
   auto pick = [&](auto al) {
-    if (vecs <= 1024)
-      go(std::integral_constant<int, 1>{}, al);
-    else
-      go(std::integral_constant<int, 4>{}, al);
+    const int nv = row_vectors(rows, vecs);
+    if (nv == 1) return go(std::integral_constant<int, 1>{}, al);
+    if (nv == 2) return go(std::integral_constant<int, 2>{}, al);
+    return go(std::integral_constant<int, 4>{}, al);
   };
-  if (aligned)
-    pick(std::true_type{});
-  else
-    pick(std::false_type{});
-  return cudaGetLastError();
+  return aligned ? pick(std::true_type{}) : pick(std::false_type{});
 }
 
 }  // namespace

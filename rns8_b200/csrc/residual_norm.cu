@@ -4,6 +4,7 @@
 
 #include "quant_common.cuh"
 #include "quant_kernels.hpp"
+#include "quant_launch.cuh"
 
 namespace rns8cuda {
 namespace {
@@ -28,6 +29,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const Forwar
   __shared__ float slots[3][32];
   const int64_t t = blockIdx.x;
   const int n = blockDim.x, tid = threadIdx.x;
+  wait_previous_launch();
+  allow_next_launch();
   float y[NV][8], x[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -105,6 +108,8 @@ template <typename T, typename W, bool ALIGNED, int NV>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const Backward p) {
   __shared__ float slots[2][6 * 32];
   const int n = blockDim.x, tid = threadIdx.x;
+  wait_previous_launch();
+  allow_next_launch();
   float acc_pre[NV][8] = {}, acc_post[NV][8] = {};
   int buf = 0;
   for (int64_t item = blockIdx.x; item < p.items; item += gridDim.x) {
@@ -225,6 +230,8 @@ struct Sums {
 __global__ void __launch_bounds__(256) sum_rows_kernel(const Sums p) {
   __shared__ float s[8][33];
   const int z = blockIdx.z;
+  wait_previous_launch();
+  allow_next_launch();
   if (!p.out[z]) return;
   const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
   for (int64_t g = blockIdx.y; g < p.groups[z]; g += gridDim.y) {
@@ -246,29 +253,25 @@ bool aligned_rows(const void* p, int64_t ld, size_t elem) {
 }
 size_t type_size(uint32_t t) { return t == RNS8_CUDA_TYPE_F32 ? 4 : 2; }
 
-int block_threads(int dim, int nv) { return std::max(32, ((dim + 7) / 8 + nv - 1) / nv); }
+unsigned block_threads(int dim, int nv) {
+  return static_cast<unsigned>(std::max(32, (((dim + 7) / 8 + nv - 1) / nv + 31) / 32 * 32));
+}
 
 // Calls f(T, W, ALIGNED, NV) as types for the descriptor's element types.
 template <typename F>
-void dispatch(uint32_t type, uint32_t weight_type, bool aligned, int dim, F&& f) {
+cudaError_t dispatch(uint32_t type, uint32_t weight_type, bool aligned, int nv, F&& f) {
   auto with = [&](auto t, auto w) {
     auto al = [&](auto a) {
-      if ((dim + 7) / 8 <= kMaxThreads)
-        f(t, w, a, std::integral_constant<int, 1>{});
-      else
-        f(t, w, a, std::integral_constant<int, 4>{});
+      if (nv == 1) return f(t, w, a, std::integral_constant<int, 1>{});
+      if (nv == 2) return f(t, w, a, std::integral_constant<int, 2>{});
+      return f(t, w, a, std::integral_constant<int, 4>{});
     };
-    if (aligned)
-      al(std::true_type{});
-    else
-      al(std::false_type{});
+    return aligned ? al(std::true_type{}) : al(std::false_type{});
   };
-  if (type == RNS8_CUDA_TYPE_F32)
-    with(float{}, float{});
-  else if (type == RNS8_CUDA_TYPE_BF16)
-    weight_type == RNS8_CUDA_TYPE_F32 ? with(__nv_bfloat16{}, float{}) : with(__nv_bfloat16{}, __nv_bfloat16{});
-  else
-    weight_type == RNS8_CUDA_TYPE_F32 ? with(__half{}, float{}) : with(__half{}, __half{});
+  if (type == RNS8_CUDA_TYPE_F32) return with(float{}, float{});
+  if (type == RNS8_CUDA_TYPE_BF16)
+    return weight_type == RNS8_CUDA_TYPE_F32 ? with(__nv_bfloat16{}, float{}) : with(__nv_bfloat16{}, __nv_bfloat16{});
+  return weight_type == RNS8_CUDA_TYPE_F32 ? with(__half{}, float{}) : with(__half{}, __half{});
 }
 
 // How the backward pass splits its tokens: items of one gate row each, at
@@ -311,13 +314,12 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t st
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.x_out, d.ld_x_out, e) &&
                        aligned_rows(d.h, d.ld_h, e) &&
                        (!d.q || (reinterpret_cast<uintptr_t>(d.q) % 8 == 0 && d.ld_q % 8 == 0));
-  dispatch(d.type, d.weight_type, aligned, p.dim, [&](auto t, auto wt, auto al, auto nv) {
+  const int vectors = row_vectors(d.tokens, (p.dim + 7) / 8);
+  return dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
-    const int threads = (block_threads(p.dim, NV) + 31) / 32 * 32;
-    residual_norm_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>
-        <<<static_cast<unsigned>(d.tokens), threads, 0, stream>>>(p);
+    return launch_chained(residual_norm_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
+                          dim3(static_cast<unsigned>(d.tokens)), block_threads(p.dim, NV), 0, 1, stream, p);
   });
-  return cudaGetLastError();
 }
 
 uint64_t residual_norm_backward_scratch_bytes(const rns8_cuda_residual_norm_backward_desc& d, int sm_count) {
@@ -372,18 +374,16 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
                        aligned_rows(d.d_y, d.ld_d_y, e) && d.dim % 4 == 0 &&
                        (!s.per_token || aligned_rows(d.d_gate, d.ld_d_gate, e));
-  dispatch(d.type, d.weight_type, aligned, p.dim, [&](auto t, auto wt, auto al, auto nv) {
+  const int vectors = (p.dim + 7) / 8 <= kMaxThreads ? 1 : 4;
+  cudaError_t err = dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
-    const int threads = (block_threads(p.dim, NV) + 31) / 32 * 32;
-    residual_norm_backward_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>
-        <<<static_cast<unsigned>(s.grid), threads, 0, stream>>>(p);
+    return launch_chained(residual_norm_backward_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
+                          dim3(static_cast<unsigned>(s.grid)), block_threads(p.dim, NV), 0, 1, stream, p);
   });
-  cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   if (sums.out[0] || sums.out[1] || sums.out[2]) {
     const unsigned gy = static_cast<unsigned>(std::min<int64_t>(sums.out[2] ? s.groups : 1, 1024));
-    sum_rows_kernel<<<dim3((p.dim + 31) / 32, gy, 3), 256, 0, stream>>>(sums);
-    err = cudaGetLastError();
+    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), 256, 0, 1, stream, sums);
   }
   return err;
 }
