@@ -134,7 +134,7 @@ extern "C" rns8_status rns8_cuda_residual_norm_device(const rns8_cuda_residual_n
     return RNS8_INVALID_ARGUMENT;
   rns8host::DeviceScope scope(d.device_id);
   if (!scope.ok) return RNS8_BACKEND_FAILURE;
-  return launch_result(rns8cuda::residual_norm(d, static_cast<cudaStream_t>(d.stream)));
+  return launch_result(rns8cuda::residual_norm(d, sm_count_of(d.device_id), static_cast<cudaStream_t>(d.stream)));
 }
 
 extern "C" uint64_t

@@ -3,10 +3,12 @@
 // quantisation rule.
 //
 // A row kernel gives every thread NV vectors of 8 elements. With ALIGNED rows
-// (base and leading dimension on 16-byte boundaries) vector v of thread t
-// covers elements 8 * (v * threads + t) .. + 7 and moves as 16-byte words;
-// otherwise its e-th element is (8 v + e) * threads + t, so that a warp's
-// element-wise accesses are contiguous. Elements past the row read as zero.
+// (whole vectors, base and leading dimension on 16-byte boundaries) vector v of
+// thread t covers elements 8 * (v * threads + t) .. + 7 and moves as 16-byte
+// words; otherwise its e-th element is (8 v + e) * threads + t, so that a
+// warp's element-wise accesses are contiguous. Elements past the row read as
+// zero. No kernel holds both forms: short calls wait for their code to arrive
+// as much as for their data.
 #pragma once
 
 #include <cfloat>
@@ -51,48 +53,133 @@ __device__ __forceinline__ int row_index(int v, int e, int threads, int tid) {
   return ALIGNED ? (v * threads + tid) * 8 + e : (v * 8 + e) * threads + tid;
 }
 
-// Eight elements as 32-bit floats; elements at or past `cols` are zero.
-template <bool ALIGNED, typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int cols, int v, int threads, int tid, float (&out)[8]) {
-  if (ALIGNED) {
-    const int i = (v * threads + tid) * 8;
-    if (i + 8 <= cols) {
-      constexpr int WORDS = static_cast<int>(sizeof(T) * 8 / 16);
-      uint4 raw[WORDS];
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) raw[w] = reinterpret_cast<const uint4*>(row + i)[w];
-      const T* t = reinterpret_cast<const T*>(raw);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = to_f32(t[e]);
-      return;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = row_index<ALIGNED>(v, e, threads, tid);
-    out[e] = i < cols ? to_f32(row[i]) : 0.0f;
-  }
+// ---- pairs of 32-bit floats ---------------------------------------------------------
+// sm_100 multiplies and adds two floats an instruction; the row kernels are as
+// much bound by issue as by HBM.
+struct F2 {
+  float2 v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) { return F2{make_float2(a, b)}; }
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ uint64_t bits(F2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v.x), "f"(a.v.y));
+  return r;
+}
+__device__ __forceinline__ F2 from_bits(uint64_t r) {
+  F2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.v.x), "=f"(a.v.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return from_bits(r);
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return from_bits(r);
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return from_bits(r);
+}
+__device__ __forceinline__ float both(F2 a) { return a.v.x + a.v.y; }
+
+// Two elements of a 16-bit type in a word, as floats and back.
+template <typename T>
+__device__ __forceinline__ F2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ F2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ F2 unpack2<__half>(uint32_t w) {
+  return F2{__half22float2(*reinterpret_cast<const __half2*>(&w))};
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(F2 a);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(F2 a) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a.v.x, a.v.y);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(F2 a) {
+  const __half2 r = __floats2half2_rn(a.v.x, a.v.y);
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Eight elements as they lie in memory: the words of an aligned vector.
+template <typename T>
+struct Raw8 {
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p, bool in) {
+    w = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ F2 pair(int i) const {
+    return unpack2<T>(i == 0 ? w.x : (i == 1 ? w.y : (i == 2 ? w.z : w.w)));
+  }
+  __device__ __forceinline__ void set(const F2 (&v)[4]) {
+    w = make_uint4(pack2<T>(v[0]), pack2<T>(v[1]), pack2<T>(v[2]), pack2<T>(v[3]));
+  }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+};
+template <>
+struct Raw8<float> {
+  float4 lo, hi;
+  __device__ __forceinline__ void load(const float* p, bool in) {
+    lo = in ? reinterpret_cast<const float4*>(p)[0] : make_float4(0, 0, 0, 0);
+    hi = in ? reinterpret_cast<const float4*>(p)[1] : make_float4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ F2 pair(int i) const {
+    return i == 0 ? f2(lo.x, lo.y) : (i == 1 ? f2(lo.z, lo.w) : (i == 2 ? f2(hi.x, hi.y) : f2(hi.z, hi.w)));
+  }
+  __device__ __forceinline__ void set(const F2 (&v)[4]) {
+    lo = make_float4(v[0].v.x, v[0].v.y, v[1].v.x, v[1].v.y);
+    hi = make_float4(v[2].v.x, v[2].v.y, v[3].v.x, v[3].v.y);
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = lo;
+    reinterpret_cast<float4*>(p)[1] = hi;
+  }
+};
+
+// Vector v of this thread's part of a row; elements at or past `cols` are zero.
 template <bool ALIGNED, typename T>
-__device__ __forceinline__ void store8(T* __restrict__ row, int cols, int v, int threads, int tid, const float (&in)[8]) {
+__device__ __forceinline__ void load8(const T* __restrict__ row, int cols, int v, int threads, int tid, F2 (&out)[4]) {
   if (ALIGNED) {
     const int i = (v * threads + tid) * 8;
-    if (i + 8 <= cols) {
-      constexpr int WORDS = static_cast<int>(sizeof(T) * 8 / 16);
-      uint4 raw[WORDS];
-      T* t = reinterpret_cast<T*>(raw);
+    Raw8<T> raw;
+    raw.load(row + i, i < cols);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(in[e]);
+    for (int e = 0; e < 4; ++e) out[e] = raw.pair(e);
+  } else {
+    float x[8];
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) reinterpret_cast<uint4*>(row + i)[w] = raw[w];
-      return;
+    for (int e = 0; e < 8; ++e) {
+      const int i = row_index<ALIGNED>(v, e, threads, tid);
+      x[e] = i < cols ? to_f32(row[i]) : 0.0f;
     }
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = row_index<ALIGNED>(v, e, threads, tid);
-    if (i < cols) row[i] = from_f32<T>(in[e]);
+    for (int e = 0; e < 4; ++e) out[e] = f2(x[2 * e], x[2 * e + 1]);
+  }
+}
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ void store8(T* __restrict__ row, int cols, int v, int threads, int tid, const F2 (&in)[4]) {
+  if (ALIGNED) {
+    const int i = (v * threads + tid) * 8;
+    Raw8<T> raw;
+    raw.set(in);
+    if (i < cols) raw.store(row + i);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = row_index<ALIGNED>(v, e, threads, tid);
+      if (i < cols) row[i] = from_f32<T>(e % 2 ? in[e / 2].v.y : in[e / 2].v.x);
+    }
   }
 }
 
@@ -127,52 +214,103 @@ __device__ __forceinline__ RowScale make_row_scale(uint32_t max_bits) {
 // product of an infinity or a NaN is a NaN, which converts to 0.
 __device__ __forceinline__ int quantize_one(float x, float inv) { return __float2int_rn(x * inv); }
 
+__device__ __forceinline__ uint32_t magnitude_bits(const F2 (&v)[4]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, max(magnitude_bits(v[e].v.x), magnitude_bits(v[e].v.y)));
+  return top;
+}
+
 template <bool ALIGNED>
 __device__ __forceinline__ void store_q8(int8_t* __restrict__ row, int cols, int v, int threads, int tid,
-                                         const float (&in)[8], float inv) {
+                                         const F2 (&in)[4], float inv) {
+  uint32_t q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = static_cast<uint32_t>(quantize_one(e % 2 ? in[e / 2].v.y : in[e / 2].v.x, inv));
   if (ALIGNED) {
     const int i = (v * threads + tid) * 8;
-    if (i + 8 <= cols) {
-      uint32_t w[2];
+    if (i < cols)
+      *reinterpret_cast<uint2*>(row + i) =
+          make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                     __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+  } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t q0 = quantize_one(in[4 * h], inv), q1 = quantize_one(in[4 * h + 1], inv);
-        const uint32_t q2 = quantize_one(in[4 * h + 2], inv), q3 = quantize_one(in[4 * h + 3], inv);
-        w[h] = __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
-      }
-      *reinterpret_cast<uint2*>(row + i) = make_uint2(w[0], w[1]);
-      return;
+    for (int e = 0; e < 8; ++e) {
+      const int i = row_index<ALIGNED>(v, e, threads, tid);
+      if (i < cols) row[i] = static_cast<int8_t>(q[e]);
     }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = row_index<ALIGNED>(v, e, threads, tid);
-    if (i < cols) row[i] = static_cast<int8_t>(quantize_one(in[e], inv));
   }
 }
 
 // ---- block reductions ---------------------------------------------------------------
-// One barrier each: every warp leaves its part in `slots` (32 words per value)
-// and then sums all of them itself. Two reductions that follow one another use
-// different slots.
+// One barrier each: every warp leaves its part in `slots` and then joins all the
+// parts itself, four at a time. Two reductions that follow one another use
+// different slots; slots of warps that the block does not have are zero
+// (clear_slots, before the first one).
+//
+// Sums of N values over a warp: while two lanes hold 2^k values each they swap
+// halves instead of adding all of them twice, so that 8 values take 9 shuffles,
+// not 40. Lane l ends with the total of value l / (32 / N2), N2 the power of
+// two from N up.
 template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float* slots) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+constexpr int pow2_of() {
+  return N <= 1 ? 1 : 2 * pow2_of<(N + 1) / 2>();
+}
+template <int N2>
+__device__ __forceinline__ float warp_sum_spread(float (&v)[N2], int lane) {
 #pragma unroll
-  for (int n = 0; n < N; ++n)
+  for (int half = N2 / 2, o = 16; o; o >>= 1) {
+    if (half) {
+      const bool up = lane & o;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xFFFFFFFFu, v[n], o);
-  if (warps == 1) return;
-  if (lane == 0)
-#pragma unroll
-    for (int n = 0; n < N; ++n) slots[n * 32 + warp] = v[n];
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    v[n] = lane < warps ? slots[n * 32 + lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xFFFFFFFFu, v[n], o);
+      for (int i = 0; i < half; ++i) {
+        const float send = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+      }
+      half >>= 1;
+    } else {
+      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+    }
   }
+  return v[0];
+}
+
+template <int N>
+struct SumSlots {
+  static constexpr int N2 = pow2_of<N>();
+  float4 part[N2][8];  // [value][warp / 4], .xyzw by warp % 4
+};
+template <int N>
+__device__ __forceinline__ void clear_slots(SumSlots<N>& s) {
+  for (int i = threadIdx.x; i < SumSlots<N>::N2 * 32; i += blockDim.x) reinterpret_cast<float*>(s.part)[i] = 0.0f;
+}
+
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], SumSlots<N>& slots) {
+  constexpr int N2 = SumSlots<N>::N2, SHARE = 32 / N2;  // lanes of a warp for each value
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  float w[N2];
+#pragma unroll
+  for (int n = 0; n < N2; ++n) w[n] = n < N ? v[n < N ? n : 0] : 0.0f;
+  float total = warp_sum_spread(w, lane);
+  if (warps > 1) {
+    if (lane % SHARE == 0) reinterpret_cast<float*>(slots.part[lane / SHARE])[warp] = total;
+    __syncthreads();
+    // Four warps' parts a lane; 8 / (lanes a value has) rounds for up to 32 warps.
+    total = 0.0f;
+#pragma unroll
+    for (int q = lane % SHARE; q < 8; q += SHARE) {
+      if (q * 4 >= warps) break;
+      const float4 f = slots.part[lane / SHARE][q];
+      total += (f.x + f.y) + (f.z + f.w);
+    }
+    // The lanes past the eighth of a value have nothing: the sum stays whole.
+#pragma unroll
+    for (int o = (SHARE < 8 ? SHARE : 8) / 2; o; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    if (SHARE > 8) total = __shfl_sync(0xFFFFFFFFu, total, lane / SHARE * SHARE);
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) v[n] = N2 == 1 ? total : __shfl_sync(0xFFFFFFFFu, total, n * SHARE);
 }
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;

@@ -16,7 +16,7 @@ cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t 
 uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d);
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream);
 
-cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t stream);
+cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, cudaStream_t stream);
 uint64_t residual_norm_backward_scratch_bytes(const rns8_cuda_residual_norm_backward_desc& d, int sm_count);
 cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& d, int sm_count, cudaStream_t stream);
 

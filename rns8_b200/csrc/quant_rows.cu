@@ -18,14 +18,12 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict
   allow_next_launch();
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ld_x;
-  float v[NV][8];
+  F2 v[NV][4];
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    load8<ALIGNED>(xr, cols, j, blockDim.x, threadIdx.x, v[j]);
+  for (int j = 0; j < NV; ++j) load8<ALIGNED>(xr, cols, j, blockDim.x, threadIdx.x, v[j]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(v[j][e]));
-  }
+  for (int j = 0; j < NV; ++j) top = max(top, magnitude_bits(v[j]));
   const RowScale rs = make_row_scale(block_max(top, slots));
   if (threadIdx.x == 0) scale[row] = rs.scale;
 #pragma unroll
@@ -52,7 +50,7 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* __res
 template <typename T>
 cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
                    cudaStream_t stream) {
-  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0 &&
+  const bool aligned = cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(q) % 8 == 0 && ld_q % 8 == 0;
   const dim3 grid(static_cast<unsigned>(rows));
   if (cols > 1024 * 8 * 4)

@@ -1,7 +1,20 @@
 // The norms around a block fused with its gate and residual update, forward
 // and backward (include/rns8/rns8_quant.h holds the formulas).
+//
+// Both directions move a few bytes per element and do some tens of operations
+// on it, so HBM is to bound them; what stands in the way is that a row must be
+// reduced before any of it can be written. Two forms each:
+//
+//   streamed  For rows on 16-byte boundaries and many tokens: persistent
+//             blocks whose rows arrive in shared memory through a ring of bulk
+//             copies, so that the next tokens' bytes are on their way while
+//             this token is reduced.
+//   direct    For the rest (unaligned rows, few tokens, very wide rows): a row
+//             read straight into registers.
 #include <algorithm>
+#include <atomic>
 
+#include "device_common.cuh"
 #include "quant_common.cuh"
 #include "quant_kernels.hpp"
 #include "quant_launch.cuh"
@@ -22,69 +35,226 @@ struct Forward {
   int dim;
 };
 
+// Sum of a row's squares over the block.
+template <int NV>
+__device__ __forceinline__ float row_squares(const F2 (&v)[NV][4], SumSlots<1>& slots) {
+  F2 s = f2(0.0f);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = fma(v[j][e], v[j][e], s);
+  float sum[1] = {both(s)};
+  block_sum(sum, slots);
+  return sum[0];
+}
+
+// x += f * y * (offset + post) * gate for one vector; f holds scale and y's row
+// factor. The options' branches are taken per vector.
+template <bool ALIGNED, typename T, typename W>
+__device__ __forceinline__ void add_update(const Forward& p, const W* gate, float f, int j, int n, int tid,
+                                           const F2 (&y)[4], F2 (&x)[4]) {
+  F2 m[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m[e] = f2(f);
+  if (p.post) {
+    F2 w[4];
+    load8<ALIGNED>(static_cast<const W*>(p.post), p.dim, j, n, tid, w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = m[e] * (w[e] + f2(p.offset));
+  }
+  if (p.gate) {
+    F2 g[4];
+    load8<ALIGNED>(gate, p.dim, j, n, tid, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = m[e] * g[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = fma(y[e], m[e], x[e]);
+}
+template <bool ALIGNED, typename W>
+__device__ __forceinline__ void normalize(const Forward& p, float rho, int j, int n, int tid, F2 (&x)[4]) {
+  F2 w[4];
+  load8<ALIGNED>(static_cast<const W*>(p.pre), p.dim, j, n, tid, w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = x[e] * (f2(rho) * (w[e] + f2(p.offset)));
+}
+// Largest magnitude of a vector. Elements past the row are left out: they are
+// zero, but a row that holds an infinity has rho = 0 or NaN.
+template <bool ALIGNED>
+__device__ __forceinline__ uint32_t row_magnitude(const F2 (&v)[4], int dim, int j, int n, int tid) {
+  if (ALIGNED) return (j * n + tid) * 8 < dim ? magnitude_bits(v) : 0u;
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (row_index<ALIGNED>(j, e, n, tid) < dim) top = max(top, magnitude_bits(e % 2 ? v[e / 2].v.y : v[e / 2].v.x));
+  return top;
+}
+
 // One block per token; the token's row stays in registers from its load to its
 // stores.
 template <typename T, typename W, bool ALIGNED, int NV>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const Forward p) {
-  __shared__ float slots[3][32];
+  __shared__ SumSlots<1> slots[2];
+  __shared__ uint32_t max_slots[32];
   const int64_t t = blockIdx.x;
   const int n = blockDim.x, tid = threadIdx.x;
+  clear_slots(slots[0]);
+  clear_slots(slots[1]);
+  __syncthreads();
   wait_previous_launch();
   allow_next_launch();
-  float y[NV][8], x[NV][8];
+  F2 y[NV][4], x[NV][4];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     load8<ALIGNED>(static_cast<const T*>(p.y) + t * p.ld_y, p.dim, j, n, tid, y[j]);
     load8<ALIGNED>(static_cast<const T*>(p.x) + t * p.ld_x, p.dim, j, n, tid, x[j]);
   }
+  const W* gate = static_cast<const W*>(p.gate) + (p.gate ? t / p.rows_per_gate * p.ld_gate : 0);
   float f = p.scale;
-  if (p.post) {
-    float s[1] = {0.0f};
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[0] += y[j][e] * y[j][e];
-    block_sum(s, slots[0]);
-    f *= rsqrtf(s[0] * p.inv_dim + p.eps);
-  }
-  float s[1] = {0.0f};
+  if (p.post) f *= rsqrtf(row_squares(y, slots[0]) * p.inv_dim + p.eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    float w[8], g[8];
-    if (p.post) load8<ALIGNED>(static_cast<const W*>(p.post), p.dim, j, n, tid, w);
-    if (p.gate) load8<ALIGNED>(static_cast<const W*>(p.gate) + t / p.rows_per_gate * p.ld_gate, p.dim, j, n, tid, g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float u = y[j][e] * f;
-      if (p.post) u *= p.offset + w[e];
-      if (p.gate) u *= g[e];
-      x[j][e] += u;
-      s[0] += x[j][e] * x[j][e];
-    }
+    add_update<ALIGNED, T, W>(p, gate, f, j, n, tid, y[j], x[j]);
     store8<ALIGNED>(static_cast<T*>(p.x_out) + t * p.ld_x_out, p.dim, j, n, tid, x[j]);
   }
   if (!p.pre) return;
-  block_sum(s, slots[1]);
-  const float rho = rsqrtf(s[0] * p.inv_dim + p.eps);
-  uint32_t top = 0;
+  const float rho = rsqrtf(row_squares(x, slots[1]) * p.inv_dim + p.eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    float w[8];
-    load8<ALIGNED>(static_cast<const W*>(p.pre), p.dim, j, n, tid, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // Elements past the row are zero and stay zero whatever rho is: a row
-      // that holds an infinity has rho = 0 or NaN, and its own elements say so.
-      x[j][e] *= rho * (p.offset + w[e]);
-      if (row_index<ALIGNED>(j, e, n, tid) < p.dim) top = max(top, magnitude_bits(x[j][e]));
-    }
+    normalize<ALIGNED, W>(p, rho, j, n, tid, x[j]);
     if (p.h) store8<ALIGNED>(static_cast<T*>(p.h) + t * p.ld_h, p.dim, j, n, tid, x[j]);
   }
   if (!p.q) return;
-  const RowScale rs = make_row_scale(block_max(top, reinterpret_cast<uint32_t*>(slots[2])));
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<ALIGNED>(x[j], p.dim, j, n, tid));
+  const RowScale rs = make_row_scale(block_max(top, max_slots));
   if (tid == 0) p.q_scale[t] = rs.scale;
 #pragma unroll
   for (int j = 0; j < NV; ++j) store_q8<ALIGNED>(p.q + t * p.ld_q, p.dim, j, n, tid, x[j], rs.inv);
+}
+
+// ---- rows through shared memory -----------------------------------------------------
+constexpr int kMaxRing = 8;
+
+// A ring of `stages` slots, each ROWS rows of row_bytes bytes, filled by one
+// thread's bulk copies. A wait that runs out cannot be reported (these calls
+// have no status word), so it does not change the result instead: the thread
+// reads its part of that and every later row from global memory.
+template <int ROWS>
+struct RowRing {
+  uint8_t* base;
+  uint64_t* full;
+  uint32_t row_bytes, stages, stage = 0, phase = 0;
+  uint32_t filled = 0, parity = ~0u;  // slots ever filled, parity of each one's last fill
+  bool lost = false;
+
+  __device__ uint8_t* slot(uint32_t s, int row) const { return base + (s * ROWS + row) * row_bytes; }
+  // One thread: the rows of one token into slot s (a null row is left out).
+  __device__ void fill(uint32_t s, const uint8_t* const (&rows)[ROWS]) {
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) bytes += rows[r] ? row_bytes : 0;
+    mbar_arrive_expect_tx(&full[s], bytes);
+    filled |= 1u << s;
+    parity ^= 1u << s;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (rows[r]) bulk_load_1d(slot(s, r), rows[r], row_bytes, &full[s]);
+  }
+  __device__ void wait() {
+    if (!lost) lost = !mbar_wait_bounded(&full[stage], phase);
+  }
+  // The filling thread, last: its copies have landed before the block exits.
+  __device__ void drain() const {
+    for (uint32_t s = 0; s < stages; ++s)
+      if (filled & (1u << s)) (void)mbar_wait_bounded(&full[s], (parity >> s) & 1u);
+  }
+  __device__ void next() {
+    if (++stage == stages) stage = 0, phase ^= 1u;
+  }
+};
+
+// The streamed forward form: dim a multiple of 8, at most NV vectors a thread.
+template <typename T, typename W, int NV>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_stream_kernel(const Forward p, int64_t tokens, uint32_t stages) {
+  extern __shared__ __align__(16) uint8_t ring_bytes[];
+  __shared__ __align__(8) uint64_t full[kMaxRing];
+  __shared__ SumSlots<1> slots[2][2];
+  __shared__ uint32_t max_slots[2][32];
+  const int n = blockDim.x, tid = threadIdx.x;
+  for (int b = 0; b < 4; ++b) clear_slots(slots[b / 2][b % 2]);
+  RowRing<2> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), stages};
+  if (tid == 0) {
+    for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  wait_previous_launch();
+  allow_next_launch();
+  const T* xs = static_cast<const T*>(p.x);
+  const T* ys = static_cast<const T*>(p.y);
+  auto fill = [&](uint32_t s, int64_t t) {
+    const uint8_t* rows[2] = {reinterpret_cast<const uint8_t*>(xs + t * p.ld_x),
+                              reinterpret_cast<const uint8_t*>(ys + t * p.ld_y)};
+    ring.fill(s, rows);
+  };
+  if (tid == 0)
+    for (uint32_t s = 0; s < stages && blockIdx.x + static_cast<int64_t>(s) * gridDim.x < tokens; ++s)
+      fill(s, blockIdx.x + static_cast<int64_t>(s) * gridDim.x);
+
+  int buf = 0;
+  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x, buf ^= 1) {
+    ring.wait();
+    F2 y[NV][4], v[NV][4];
+    Raw8<T> x[NV];
+    auto take = [&](const T* xrow, const T* yrow) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * n + tid) * 8;
+        load8<true>(yrow, p.dim, j, n, tid, y[j]);
+        x[j].load(xrow + i, i < p.dim);
+      }
+    };
+    if (!ring.lost)  // two branches, so that these are shared-memory loads
+      take(reinterpret_cast<const T*>(ring.slot(ring.stage, 0)), reinterpret_cast<const T*>(ring.slot(ring.stage, 1)));
+    else
+      take(xs + t * p.ld_x, ys + t * p.ld_y);
+    release_stage_reads();
+    // The reduction's barrier also tells the filling thread that the slot is
+    // read, so it runs without a norm of y too.
+    const float squares = row_squares(y, slots[buf][0]);
+    if (n == 32) __syncwarp();
+    const float f = p.post ? p.scale * rsqrtf(squares * p.inv_dim + p.eps) : p.scale;
+    if (tid == 0 && !ring.lost && t + static_cast<int64_t>(stages) * gridDim.x < tokens)
+      fill(ring.stage, t + static_cast<int64_t>(stages) * gridDim.x);
+    ring.next();
+
+    const W* gate = static_cast<const W*>(p.gate) + (p.gate ? t / p.rows_per_gate * p.ld_gate : 0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = x[j].pair(e);
+      add_update<true, T, W>(p, gate, f, j, n, tid, y[j], v[j]);
+      store8<true>(static_cast<T*>(p.x_out) + t * p.ld_x_out, p.dim, j, n, tid, v[j]);
+    }
+    if (!p.pre) continue;
+    const float rho = rsqrtf(row_squares(v, slots[buf][1]) * p.inv_dim + p.eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      normalize<true, W>(p, rho, j, n, tid, v[j]);
+      if (p.h) store8<true>(static_cast<T*>(p.h) + t * p.ld_h, p.dim, j, n, tid, v[j]);
+    }
+    if (!p.q) continue;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<true>(v[j], p.dim, j, n, tid));
+    const RowScale rs = make_row_scale(block_max(top, max_slots[buf]));
+    if (tid == 0) p.q_scale[t] = rs.scale;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) store_q8<true>(p.q + t * p.ld_q, p.dim, j, n, tid, v[j], rs.inv);
+  }
+  if (tid == 0) ring.drain();
 }
 
 struct Backward {
@@ -98,24 +268,103 @@ struct Backward {
   bool per_token;  // one gate row per token: d_gate is written token by token
 };
 
+// What the two backward forms share, for one vector of a row.
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ void load_or(const T* row, float none, int dim, int j, int n, int tid, F2 (&v)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = f2(none);
+  if (row) load8<ALIGNED>(row, dim, j, n, tid, v);
+}
+// a = scale * gate * (offset + post), pre = offset + pre_weight (0 without).
+template <bool ALIGNED, typename W>
+__device__ __forceinline__ void make_factors(const Backward& p, const W* gate, int j, int n, int tid, F2 (&a)[4],
+                                             F2 (&pre)[4]) {
+  F2 w[4], g[4];
+  load_or<ALIGNED>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<ALIGNED>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
+  load_or<ALIGNED>(static_cast<const W*>(p.pre), -p.offset, p.dim, j, n, tid, pre);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    a[e] = f2(p.scale) * g[e] * (w[e] + f2(p.offset));
+    pre[e] = pre[e] + f2(p.offset);
+  }
+}
+// u dx summed or single -> the gate's gradient in place, post's share added.
+template <bool ALIGNED, typename W>
+__device__ __forceinline__ void gate_gradient(const Backward& p, const W* gate, int j, int n, int tid, F2 (&udx)[4],
+                                              F2 (&acc_post)[4]) {
+  F2 w[4], g[4];
+  load_or<ALIGNED>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<ALIGNED>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    acc_post[e] = fma(f2(p.scale) * g[e], udx[e], acc_post[e]);
+    udx[e] = f2(p.scale) * (w[e] + f2(p.offset)) * udx[e];
+  }
+}
+// A row needs one reduction: with a = scale * gate * (offset + post),
+// mean(v u) expands over dx = dxo + rho t - rho^2 mean(t n) x into sums that do
+// not depend on dx.
+struct RowSums {
+  F2 xx, tx, yy, yd, yt, yx;
+  __device__ __forceinline__ void add(const F2 (&dxo)[4], const F2 (&dh)[4], const F2 (&x)[4], const F2 (&y)[4],
+                                      const F2 (&a)[4], const F2 (&pre)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const F2 t = dh[e] * pre[e], ay = a[e] * y[e];
+      xx = fma(x[e], x[e], xx);
+      tx = fma(t, x[e], tx);
+      yy = fma(y[e], y[e], yy);
+      yd = fma(ay, dxo[e], yd);
+      yt = fma(ay, t, yt);
+      yx = fma(ay, x[e], yx);
+    }
+  }
+};
+struct RowFactors {
+  F2 rho, along, sigma, back;  // 1/rms(x), -rho^2 mean(t n), 1/rms(y), -sigma^2 mean(v u)
+};
+__device__ __forceinline__ RowFactors row_factors(const Backward& p, const RowSums& sums, SumSlots<6>& slots) {
+  float s[6] = {both(sums.xx), both(sums.tx), both(sums.yy), both(sums.yd), both(sums.yt), both(sums.yx)};
+  block_sum(s, slots);
+  const float rho = p.pre ? rsqrtf(s[0] * p.inv_dim + p.eps) : 0.0f;
+  const float along = rho * rho * rho * s[1] * p.inv_dim;
+  const float sigma = p.post ? rsqrtf(s[2] * p.inv_dim + p.eps) : 1.0f;
+  const float mvu = p.post ? sigma * (s[3] + rho * s[4] - along * s[5]) * p.inv_dim : 0.0f;
+  return RowFactors{f2(rho), f2(-along), f2(sigma), f2(-sigma * sigma * mvu)};
+}
+__device__ __forceinline__ void row_gradients(const RowFactors& r, const F2 (&dxo)[4], const F2 (&dh)[4],
+                                              const F2 (&x)[4], const F2 (&y)[4], const F2 (&a)[4], const F2 (&pre)[4],
+                                              F2 (&dx)[4], F2 (&dy)[4], F2 (&udx)[4], F2 (&acc_pre)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const F2 rdh = r.rho * dh[e];
+    dx[e] = fma(r.along, x[e], fma(rdh, pre[e], dxo[e]));
+    acc_pre[e] = fma(rdh, x[e], acc_pre[e]);
+    const F2 sdx = r.sigma * dx[e];
+    dy[e] = fma(a[e], sdx, r.back * y[e]);
+    udx[e] = y[e] * sdx;
+  }
+}
+
 // A block walks items (runs of tokens that share a gate row) and keeps the
 // sums over tokens in registers: for dgate and dpost A = sum of u * dx over an
 // item (both are multiples of it by per-channel factors), for dpre its own.
-// The row needs one reduction: with a = scale * gate * (offset + post),
-// mean(v u) expands over dx = dxo + rho t - rho^2 mean(t n) x into sums that do
-// not depend on dx.
 template <typename T, typename W, bool ALIGNED, int NV>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const Backward p) {
-  __shared__ float slots[2][6 * 32];
+  __shared__ SumSlots<6> slots[2];
   const int n = blockDim.x, tid = threadIdx.x;
+  clear_slots(slots[0]);
+  clear_slots(slots[1]);
+  __syncthreads();
   wait_previous_launch();
   allow_next_launch();
-  float acc_pre[NV][8] = {}, acc_post[NV][8] = {};
+  F2 acc_pre[NV][4] = {}, acc_post[NV][4] = {};
   int buf = 0;
   for (int64_t item = blockIdx.x; item < p.items; item += gridDim.x) {
     const int64_t group = item / p.chunks, first = group * p.rows_per_group + (item % p.chunks) * p.rows_per_item;
     const int64_t last = min(first + p.rows_per_item, (group + 1) * p.rows_per_group);
-    float acc[NV][8] = {};
+    F2 acc[NV][4] = {};
     for (int64_t t = first; t < last; ++t, buf ^= 1) {
       const T* dxo = p.dxo ? static_cast<const T*>(p.dxo) + t * p.ld_dxo : nullptr;
       const T* dh = p.dh ? static_cast<const T*>(p.dh) + t * p.ld_dh : nullptr;
@@ -123,90 +372,50 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       const T* y = static_cast<const T*>(p.y) + t * p.ld_y;
       const W* gate = p.gate ? static_cast<const W*>(p.gate) + t / p.rows_per_gate * p.ld_gate : nullptr;
       struct Vec {
-        float dxo[8], dh[8], x[8], y[8], a[8], g[8], w[8], pre[8];
+        F2 dxo[4], dh[4], x[4], y[4], a[4], pre[4];
       };
       auto load = [&](int j, Vec& v) {
         load8<ALIGNED>(x, p.dim, j, n, tid, v.x);
         load8<ALIGNED>(y, p.dim, j, n, tid, v.y);
-        if (dxo) load8<ALIGNED>(dxo, p.dim, j, n, tid, v.dxo);
-        if (dh) load8<ALIGNED>(dh, p.dim, j, n, tid, v.dh);
-        if (p.pre) load8<ALIGNED>(static_cast<const W*>(p.pre), p.dim, j, n, tid, v.pre);
-        if (p.post) load8<ALIGNED>(static_cast<const W*>(p.post), p.dim, j, n, tid, v.w);
-        if (gate) load8<ALIGNED>(gate, p.dim, j, n, tid, v.g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!dxo) v.dxo[e] = 0.0f;
-          if (!dh) v.dh[e] = 0.0f;
-          v.pre[e] = p.pre ? p.offset + v.pre[e] : 0.0f;
-          v.w[e] = p.post ? p.offset + v.w[e] : 1.0f;
-          v.g[e] = gate ? p.scale * v.g[e] : p.scale;
-          v.a[e] = v.g[e] * v.w[e];
-        }
+        load_or<ALIGNED>(dxo, 0.0f, p.dim, j, n, tid, v.dxo);
+        load_or<ALIGNED>(dh, 0.0f, p.dim, j, n, tid, v.dh);
+        make_factors<ALIGNED, W>(p, gate, j, n, tid, v.a, v.pre);
       };
-      Vec v0;
-      float s[6] = {};
+      Vec v;
+      RowSums sums{};
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        load(j, v0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float th = v0.dh[e] * v0.pre[e], ay = v0.a[e] * v0.y[e];
-          s[0] += v0.x[e] * v0.x[e];
-          s[1] += th * v0.x[e];
-          s[2] += v0.y[e] * v0.y[e];
-          s[3] += ay * v0.dxo[e];
-          s[4] += ay * th;
-          s[5] += ay * v0.x[e];
-        }
+        load(j, v);
+        sums.add(v.dxo, v.dh, v.x, v.y, v.a, v.pre);
       }
-      block_sum(s, slots[buf]);
-      const float rho = p.pre ? rsqrtf(s[0] * p.inv_dim + p.eps) : 0.0f;
-      const float along = rho * rho * rho * s[1] * p.inv_dim;  // rho^2 mean(t n)
-      const float sigma = p.post ? rsqrtf(s[2] * p.inv_dim + p.eps) : 1.0f;
-      const float mvu = p.post ? sigma * (s[3] + rho * s[4] - along * s[5]) * p.inv_dim : 0.0f;
+      const RowFactors r = row_factors(p, sums, slots[buf]);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (NV > 1) load(j, v0);
-        float dx[8], dy[8], dg[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          dx[e] = v0.dxo[e] + rho * (v0.dh[e] * v0.pre[e]) - along * v0.x[e];
-          const float u = v0.y[e] * sigma;
-          dy[e] = sigma * (v0.a[e] * dx[e] - u * mvu);
-          acc_pre[j][e] += v0.dh[e] * (v0.x[e] * rho);
-          const float udx = u * dx[e];
-          if (p.per_token) {
-            dg[e] = p.scale * v0.w[e] * udx;
-            acc_post[j][e] += v0.g[e] * udx;
-          } else {
-            acc[j][e] += udx;
-          }
-        }
+        if (NV > 1) load(j, v);
+        F2 dx[4], dy[4], udx[4];
+        row_gradients(r, v.dxo, v.dh, v.x, v.y, v.a, v.pre, dx, dy, udx, acc_pre[j]);
         store8<ALIGNED>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
         store8<ALIGNED>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
-        if (p.per_token && p.dgate) store8<ALIGNED>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, dg);
+        if (p.per_token) {
+          gate_gradient<ALIGNED, W>(p, gate, j, n, tid, udx, acc_post[j]);
+          if (p.dgate) store8<ALIGNED>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
+        }
       }
     }
     if (!p.per_token) {
+      const W* gate = static_cast<const W*>(p.gate) + (p.gate ? first / p.rows_per_gate * p.ld_gate : 0);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        float w[8], g[8], dg[8];
-        if (p.post) load8<ALIGNED>(static_cast<const W*>(p.post), p.dim, j, n, tid, w);
-        if (p.gate) load8<ALIGNED>(static_cast<const W*>(p.gate) + first / p.rows_per_gate * p.ld_gate, p.dim, j, n, tid, g);
+        gate_gradient<ALIGNED, W>(p, gate, j, n, tid, acc[j], acc_post[j]);
+        float* out = p.part_gate ? p.part_gate + item * p.dim
+                                 : (p.dgate ? static_cast<float*>(p.dgate) + group * p.ld_dgate : nullptr);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          dg[e] = p.scale * (p.post ? p.offset + w[e] : 1.0f) * acc[j][e];
-          acc_post[j][e] += (p.gate ? p.scale * g[e] : p.scale) * acc[j][e];
-        }
-        if (p.part_gate) {
-          store8<ALIGNED>(p.part_gate + item * p.dim, p.dim, j, n, tid, dg);
-        } else if (p.dgate) {
-          float* out = static_cast<float*>(p.dgate) + group * p.ld_dgate;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = row_index<ALIGNED>(j, e, n, tid);
-            if (i < p.dim) out[i] = dg[e];
-          }
+          const int i = row_index<ALIGNED>(j, e, n, tid);
+          if (out && i < p.dim) out[i] = e % 2 ? acc[j][e / 2].v.y : acc[j][e / 2].v.x;
         }
       }
     }
@@ -218,8 +427,210 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   }
 }
 
+// The streamed backward form. Per element it does some 30 operations for 12
+// bytes, half of what an SM can issue at its share of HBM, so the token's words
+// are read once and the per-channel factors are made once while the gate row
+// lasts, in shared memory (a thread reads back its own, conflict-free); the
+// registers hold the row and two sums a channel. NV vectors a thread keep what
+// a row costs besides its elements (one reduction of six sums) small.
+// With a gate row per token (PER_TOKEN) the gate's words are read beside the
+// token's, and the factors kept are those of the weights alone.
+template <typename T, typename W, int NV, bool PER_TOKEN>
+__global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(const Backward p, uint32_t stages) {
+  extern __shared__ __align__(16) uint8_t ring_bytes[];
+  __shared__ __align__(8) uint64_t full[kMaxRing];
+  __shared__ SumSlots<6> slots[2];
+  const int n = blockDim.x, tid = threadIdx.x;
+  clear_slots(slots[0]);
+  clear_slots(slots[1]);
+  RowRing<4> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), stages};
+  float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * 4 * ring.row_bytes);  // [NV][4][n]: a, a, pre, pre
+  if (tid == 0) {
+    for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  wait_previous_launch();
+  allow_next_launch();
+
+  // This block's tokens in order: runs of rows_per_item from its items.
+  struct Cursor {
+    int item, t, last;
+  };
+  const int items = static_cast<int>(p.items), chunks = static_cast<int>(p.chunks);
+  auto enter = [&](Cursor& c) {
+    if (c.item >= items) return;
+    const int group = c.item / chunks;
+    c.t = static_cast<int>(group * p.rows_per_group + (c.item - group * chunks) * p.rows_per_item);
+    c.last = static_cast<int>(min(c.t + p.rows_per_item, (group + 1) * p.rows_per_group));
+  };
+  auto advance = [&](Cursor& c) {
+    if (++c.t == c.last) {
+      c.item += gridDim.x;
+      enter(c);
+    }
+  };
+  const T* dxo_base = static_cast<const T*>(p.dxo);
+  const T* dh_base = static_cast<const T*>(p.dh);
+  const T* x_base = static_cast<const T*>(p.x);
+  const T* y_base = static_cast<const T*>(p.y);
+  auto fill = [&](uint32_t s, int64_t t) {
+    const uint8_t* rows[4] = {reinterpret_cast<const uint8_t*>(dxo_base ? dxo_base + t * p.ld_dxo : nullptr),
+                              reinterpret_cast<const uint8_t*>(dh_base ? dh_base + t * p.ld_dh : nullptr),
+                              reinterpret_cast<const uint8_t*>(x_base + t * p.ld_x),
+                              reinterpret_cast<const uint8_t*>(y_base + t * p.ld_y)};
+    ring.fill(s, rows);
+  };
+  Cursor ahead{static_cast<int>(blockIdx.x), 0, 0};
+  if (tid == 0) {
+    enter(ahead);
+    for (uint32_t s = 0; s < stages && ahead.item < items; ++s, advance(ahead)) fill(s, ahead.t);
+  }
+
+  // The factors of this thread's channels in shared memory, read back by it alone.
+  auto keep_factors = [&](int t) {
+    const W* gate = PER_TOKEN || !p.gate ? nullptr : static_cast<const W*>(p.gate) + t / p.rows_per_gate * p.ld_gate;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      F2 a[4], pre[4];
+      make_factors<true, W>(p, gate, j, n, tid, a, pre);
+      float4* f = factors + j * 4 * n + tid;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f[h * n] = make_float4(a[2 * h].v.x, a[2 * h].v.y, a[2 * h + 1].v.x, a[2 * h + 1].v.y);
+        f[(2 + h) * n] = make_float4(pre[2 * h].v.x, pre[2 * h].v.y, pre[2 * h + 1].v.x, pre[2 * h + 1].v.y);
+      }
+    }
+  };
+  auto get_factors = [&](int j, F2 (&a)[4], F2 (&pre)[4]) {
+    const float4* f = factors + j * 4 * n + tid;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 fa = f[h * n], fp = f[(2 + h) * n];
+      a[2 * h] = f2(fa.x, fa.y), a[2 * h + 1] = f2(fa.z, fa.w);
+      pre[2 * h] = f2(fp.x, fp.y), pre[2 * h + 1] = f2(fp.z, fp.w);
+    }
+  };
+  F2 acc_pre[NV][4] = {}, acc[NV][4] = {};
+  int buf = 0;
+  Cursor now{static_cast<int>(blockIdx.x), 0, 0};
+  enter(now);
+  bool fresh = true;  // the gate row changed
+  while (now.item < items) {
+    const int item = now.item;
+    const int64_t t = now.t;
+    if (fresh) keep_factors(now.t);
+    Raw8<W> gate_row[PER_TOKEN ? NV : 1];
+    if (PER_TOKEN)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * n + tid) * 8;
+        gate_row[j].load(static_cast<const W*>(p.gate) + t * p.ld_gate + i, i < p.dim);
+      }
+    ring.wait();
+    Raw8<T> dxo[NV], dh[NV], x[NV], y[NV];
+    auto take = [&](const T* r0, const T* r1, const T* r2, const T* r3) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * n + tid) * 8;
+        dxo[j].load(r0 + i, i < p.dim && dxo_base);
+        dh[j].load(r1 + i, i < p.dim && dh_base);
+        x[j].load(r2 + i, i < p.dim);
+        y[j].load(r3 + i, i < p.dim);
+      }
+    };
+    auto slot = [&](int r) { return reinterpret_cast<const T*>(ring.slot(ring.stage, r)); };
+    if (!ring.lost)  // two branches, so that these are shared-memory loads
+      take(slot(0), slot(1), slot(2), slot(3));
+    else
+      take(dxo_base + t * p.ld_dxo, dh_base + t * p.ld_dh, x_base + t * p.ld_x, y_base + t * p.ld_y);
+    release_stage_reads();
+    RowSums sums{};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      F2 fdxo[4], fdh[4], fx[4], fy[4], a[4], pre[4];
+      get_factors(j, a, pre);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        fdxo[e] = dxo[j].pair(e), fdh[e] = dh[j].pair(e), fx[e] = x[j].pair(e), fy[e] = y[j].pair(e);
+      if (PER_TOKEN)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = a[e] * gate_row[j].pair(e);
+      sums.add(fdxo, fdh, fx, fy, a, pre);
+    }
+    const RowFactors r = row_factors(p, sums, slots[buf]);
+    buf ^= 1;
+    if (n == 32) __syncwarp();
+    if (tid == 0 && !ring.lost && ahead.item < items) {
+      fill(ring.stage, ahead.t);
+      advance(ahead);
+    }
+    ring.next();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      F2 dx[4], dy[4], udx[4];
+      {
+        F2 fdxo[4], fdh[4], fx[4], fy[4], a[4], pre[4];
+        get_factors(j, a, pre);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          fdxo[e] = dxo[j].pair(e), fdh[e] = dh[j].pair(e), fx[e] = x[j].pair(e), fy[e] = y[j].pair(e);
+        if (PER_TOKEN)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = a[e] * gate_row[j].pair(e);
+        row_gradients(r, fdxo, fdh, fx, fy, a, pre, dx, dy, udx, acc_pre[j]);
+      }
+      store8<true>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
+      store8<true>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
+      if (PER_TOKEN) {
+        F2 base[4], pre[4];  // scale * (offset + post)
+        get_factors(j, base, pre);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[j][e] = fma(f2(p.scale) * gate_row[j].pair(e), udx[e], acc[j][e]);
+          udx[e] = base[e] * udx[e];
+        }
+        if (p.dgate) store8<true>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
+      }
+    }
+    advance(now);
+    const bool ended = now.item != item;
+    fresh = !PER_TOKEN && ended;
+    if (PER_TOKEN || !ended) continue;
+    // The item's sums: its gate row's gradient, and its share of post's, which
+    // the block adds up over its items in its own row of part_post.
+    const W* gate = static_cast<const W*>(p.gate) + (p.gate ? t / p.rows_per_gate * p.ld_gate : 0);
+    float* dp = p.part_post ? p.part_post + static_cast<int64_t>(blockIdx.x) * p.dim : nullptr;
+    float* dg = p.part_gate ? p.part_gate + static_cast<int64_t>(item) * p.dim
+                            : (p.dgate ? static_cast<float*>(p.dgate) + item / chunks * p.ld_dgate : nullptr);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * n + tid) * 8;
+      F2 post[4] = {};
+      if (dp && item != static_cast<int>(blockIdx.x)) load8<true>(dp, p.dim, j, n, tid, post);
+      gate_gradient<true, W>(p, gate, j, n, tid, acc[j], post);
+      if (dp) store8<true>(dp, p.dim, j, n, tid, post);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (dg && i < p.dim) dg[i + 2 * e] = acc[j][e].v.x, dg[i + 2 * e + 1] = acc[j][e].v.y;
+        acc[j][e] = f2(0.0f);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (p.part_post && PER_TOKEN)
+      store8<true>(p.part_post + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc[j]);
+    if (p.part_pre) store8<true>(p.part_pre + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc_pre[j]);
+  }
+  if (tid == 0) ring.drain();
+}
+
 // out[g][c] = sum over the group's `count` consecutive rows of part. A block
-// sums 32 columns with 8 row lanes, always in the same order. blockIdx.z picks
+// sums 32 columns with 16 row lanes, always in the same order. blockIdx.z picks
 // one of three sums.
 struct Sums {
   const float* part[3];
@@ -227,22 +638,31 @@ struct Sums {
   int64_t count[3], groups[3], ld_out[3];
   int dim;
 };
-__global__ void __launch_bounds__(256) sum_rows_kernel(const Sums p) {
-  __shared__ float s[8][33];
+constexpr int kSumLanes = 16;
+__global__ void __launch_bounds__(32 * kSumLanes) sum_rows_kernel(const Sums p) {
+  __shared__ float s[kSumLanes][33];
   const int z = blockIdx.z;
   wait_previous_launch();
   allow_next_launch();
   if (!p.out[z]) return;
   const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
   for (int64_t g = blockIdx.y; g < p.groups[z]; g += gridDim.y) {
-    float v = 0.0f;
-    if (c < p.dim)
-      for (int64_t r = lane; r < p.count[z]; r += 8) v += p.part[z][(g * p.count[z] + r) * p.dim + c];
-    s[lane][threadIdx.x % 32] = v;
+    float v[4] = {};
+    const float* part = p.part[z] + g * p.count[z] * p.dim + c;
+    if (c < p.dim) {
+      int64_t r = lane;
+      for (; r + 3 * kSumLanes < p.count[z]; r += 4 * kSumLanes)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += part[(r + i * kSumLanes) * p.dim];
+      for (; r < p.count[z]; r += kSumLanes) v[0] += part[r * p.dim];
+    }
+    s[lane][threadIdx.x % 32] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
     if (lane == 0 && c < p.dim) {
-      for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
-      p.out[z][g * p.ld_out[z] + c] = v;
+      float all = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSumLanes; ++i) all += s[i][threadIdx.x];
+      p.out[z][g * p.ld_out[z] + c] = all;
     }
     __syncthreads();
   }
@@ -274,6 +694,55 @@ cudaError_t dispatch(uint32_t type, uint32_t weight_type, bool aligned, int nv, 
   return weight_type == RNS8_CUDA_TYPE_F32 ? with(__half{}, float{}) : with(__half{}, __half{});
 }
 
+// Calls f(T, W).
+template <typename F>
+cudaError_t dispatch_types(uint32_t type, uint32_t weight_type, F&& f) {
+  if (type == RNS8_CUDA_TYPE_F32) return f(float{}, float{});
+  if (type == RNS8_CUDA_TYPE_BF16)
+    return weight_type == RNS8_CUDA_TYPE_F32 ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
+  return weight_type == RNS8_CUDA_TYPE_F32 ? f(__half{}, float{}) : f(__half{}, __half{});
+}
+
+// A streamed kernel's launch: vectors and threads a block, blocks an SM (by
+// the registers those take), slots of the ring.
+struct Stream {
+  int nv;
+  unsigned threads, per_sm, stages;
+  size_t smem;
+};
+constexpr size_t kSmemOfSm = 220 * 1024;  // for the dynamic shared memory of an SM's blocks
+// The forward ring stays small: HBM needs some 45 KB of an SM in flight, and
+// the rest of the SM's memory caches the weights, which every token reads
+// again (8192 x 8192 bf16: 97 us; 111 us with a ring of three rows a block).
+constexpr size_t kForwardSmemOfSm = 64 * 1024;
+
+Stream forward_stream(int dim, size_t elem) {
+  const int vecs = dim / 8;
+  Stream s{};
+  s.nv = vecs <= 32 ? 1 : 2;
+  s.threads = block_threads(dim, s.nv);
+  s.per_sm = std::max(1u, std::min(16u, 1024 / s.threads));
+  const size_t slot = 2 * static_cast<size_t>(dim) * elem;
+  s.stages = static_cast<unsigned>(std::min<size_t>(kMaxRing, std::max<size_t>(1, kForwardSmemOfSm / s.per_sm / slot)));
+  s.smem = s.stages * slot;
+  return s;
+}
+
+// The backward pass. Its grid depends on the sizes alone, so that the scratch
+// for the blocks' sums does too.
+Stream backward_stream(int dim, size_t elem) {
+  const int vecs = (dim + 7) / 8;
+  Stream s{};
+  s.nv = vecs <= 64 ? 1 : 2;
+  s.threads = block_threads(dim, s.nv);
+  s.per_sm = std::max(1u, std::min(8u, 512 / s.threads));
+  const size_t slot = 4 * static_cast<size_t>(dim) * elem, factors = 64 * static_cast<size_t>(s.nv) * s.threads;
+  const size_t room = kSmemOfSm / s.per_sm;
+  s.stages = static_cast<unsigned>(room > factors ? std::min<size_t>(kMaxRing, (room - factors) / slot) : 0);
+  s.smem = s.stages * slot + factors;
+  return s;
+}
+
 // How the backward pass splits its tokens: items of one gate row each, at
 // most `chunks` items per gate row, walked by `grid` blocks.
 struct Split {
@@ -283,7 +752,8 @@ struct Split {
 };
 Split split_tokens(const rns8_cuda_residual_norm_backward_desc& d, int sm_count) {
   Split s;
-  const int64_t target = 2 * static_cast<int64_t>(sm_count);
+  const Stream st = backward_stream(static_cast<int>(d.dim), type_size(d.type));
+  const int64_t target = static_cast<int64_t>(st.per_sm) * sm_count;
   s.per_token = d.gate && d.groups == d.tokens;
   s.groups = (s.per_token || !d.gate) ? 1 : d.groups;
   s.rows_per_group = d.tokens / s.groups;
@@ -300,7 +770,7 @@ bool gate_partials(const rns8_cuda_residual_norm_backward_desc& d, const Split& 
 
 }  // namespace
 
-cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t stream) {
+cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, cudaStream_t stream) {
   Forward p{};
   p.rows_per_gate = d.gate ? d.tokens / d.groups : 1;
   p.ld_x = d.ld_x, p.ld_y = d.ld_y, p.ld_gate = d.ld_gate, p.ld_x_out = d.ld_x_out, p.ld_h = d.ld_h, p.ld_q = d.ld_q;
@@ -309,11 +779,29 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, cudaStream_t st
   p.scale = d.scale, p.eps = d.eps, p.offset = d.weight_offset, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
   const size_t e = type_size(d.type), w = type_size(d.weight_type);
-  const bool aligned = aligned_rows(d.x, d.ld_x, e) && aligned_rows(d.y, d.ld_y, e) &&
+  const bool aligned = d.dim % 8 == 0 && aligned_rows(d.x, d.ld_x, e) && aligned_rows(d.y, d.ld_y, e) &&
                        aligned_rows(d.post_weight, 0, w) && aligned_rows(d.pre_weight, 0, w) &&
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.x_out, d.ld_x_out, e) &&
                        aligned_rows(d.h, d.ld_h, e) &&
                        (!d.q || (reinterpret_cast<uintptr_t>(d.q) % 8 == 0 && d.ld_q % 8 == 0));
+  // Below some four tokens an SM each block has one or two rows and nothing to
+  // run ahead for: the direct form's shorter start wins.
+  if (aligned && p.dim <= 16384 && d.tokens >= 4 * static_cast<int64_t>(sm_count)) {
+    const Stream s = forward_stream(p.dim, e);
+    auto launch_stream = [&](auto t, auto wt, auto nv) {
+      auto kernel = residual_norm_stream_kernel<decltype(t), decltype(wt), decltype(nv)::value>;
+      static std::atomic<uint64_t> configured{0};
+      const cudaError_t err = raise_smem_limit_once(kernel, static_cast<int>(kSmemOfSm), configured);
+      if (err != cudaSuccess) return err;
+      const int64_t grid = std::min<int64_t>(d.tokens, static_cast<int64_t>(s.per_sm) * sm_count);
+      return launch_chained(kernel, dim3(static_cast<unsigned>(grid)), s.threads, s.smem, 1, stream, p, d.tokens,
+                            s.stages);
+    };
+    return dispatch_types(d.type, d.weight_type, [&](auto t, auto wt) {
+      return s.nv == 1 ? launch_stream(t, wt, std::integral_constant<int, 1>{})
+                       : launch_stream(t, wt, std::integral_constant<int, 2>{});
+    });
+  }
   const int vectors = row_vectors(d.tokens, (p.dim + 7) / 8);
   return dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
@@ -368,14 +856,29 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   }
 
   const size_t e = type_size(d.type), w = type_size(d.weight_type);
-  const bool aligned = aligned_rows(d.d_x_out, d.ld_d_x_out, e) && aligned_rows(d.d_h, d.ld_d_h, e) &&
+  const bool aligned = d.dim % 8 == 0 && aligned_rows(d.d_x_out, d.ld_d_x_out, e) && aligned_rows(d.d_h, d.ld_d_h, e) &&
                        aligned_rows(d.x_out, d.ld_x_out, e) && aligned_rows(d.y, d.ld_y, e) &&
                        aligned_rows(d.post_weight, 0, w) && aligned_rows(d.pre_weight, 0, w) &&
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
-                       aligned_rows(d.d_y, d.ld_d_y, e) && d.dim % 4 == 0 &&
+                       aligned_rows(d.d_y, d.ld_d_y, e) &&
                        (!s.per_token || aligned_rows(d.d_gate, d.ld_d_gate, e));
+  const Stream st = backward_stream(p.dim, e);
+  const bool streamed = aligned && p.dim <= 8192 && st.stages > 0;
   const int vectors = (p.dim + 7) / 8 <= kMaxThreads ? 1 : 4;
-  cudaError_t err = dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
+  auto launch_stream = [&](auto t, auto wt, auto nv, auto per_token) {
+    auto kernel =
+        residual_norm_backward_stream_kernel<decltype(t), decltype(wt), decltype(nv)::value, decltype(per_token)::value>;
+    static std::atomic<uint64_t> configured{0};
+    const cudaError_t bad = raise_smem_limit_once(kernel, static_cast<int>(kSmemOfSm), configured);
+    if (bad != cudaSuccess) return bad;
+    return launch_chained(kernel, dim3(static_cast<unsigned>(s.grid)), st.threads, st.smem, 1, stream, p, st.stages);
+  };
+  cudaError_t err = streamed ? dispatch_types(d.type, d.weight_type, [&](auto t, auto wt) {
+    auto go = [&](auto nv) {
+      return s.per_token ? launch_stream(t, wt, nv, std::true_type{}) : launch_stream(t, wt, nv, std::false_type{});
+    };
+    return st.nv == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
+  }) : dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
     return launch_chained(residual_norm_backward_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
                           dim3(static_cast<unsigned>(s.grid)), block_threads(p.dim, NV), 0, 1, stream, p);
@@ -383,7 +886,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   if (err != cudaSuccess) return err;
   if (sums.out[0] || sums.out[1] || sums.out[2]) {
     const unsigned gy = static_cast<unsigned>(std::min<int64_t>(sums.out[2] ? s.groups : 1, 1024));
-    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), 256, 0, 1, stream, sums);
+    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), 32 * kSumLanes, 0, 1, stream, sums);
   }
   return err;
 }
