@@ -13,20 +13,34 @@ namespace {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
 
-// dst rows (ld a multiple of 16) from src rows of any alignment. Bytes past
-// cols are zero.
+// dst rows (ld a multiple of 16) from src rows of any alignment, 16 bytes a
+// thread: the five aligned words around them, shifted into place (1001 x 2040:
+// 3.7 us byte by byte). Bytes past cols are zero; where a word would reach
+// outside the matrix the bytes are read one by one.
 __global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ src, int64_t rows, int64_t cols,
                                                          int64_t ld, int8_t* __restrict__ dst, int64_t ld_dst) {
   wait_previous_launch();
   allow_next_launch();
   const int64_t per_row = ld_dst / 16, total = rows * per_row;
+  const int8_t* end = src + (rows - 1) * ld + cols;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+    const int8_t* from = src + r * ld + c;
+    const uint32_t shift = reinterpret_cast<uintptr_t>(from) % 4 * 8;
+    const int8_t* base = from - shift / 8;
     uint32_t w[4] = {0, 0, 0, 0};
+    if (c + 16 <= cols && base >= src && base + 20 <= end) {
+      uint32_t v[5];
 #pragma unroll
-    for (int b = 0; b < 16; ++b)
-      if (c + b < cols) w[b / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(src[r * ld + c + b])) << (8 * (b % 4));
+      for (int k = 0; k < 5; ++k) v[k] = reinterpret_cast<const uint32_t*>(base)[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], shift);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 16; ++b)
+        if (c + b < cols) w[b / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[b])) << (8 * (b % 4));
+    }
     *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }

@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 
 #include "device_common.cuh"
@@ -53,18 +54,21 @@ __device__ __forceinline__ void report_timeout(const TcLinear& p, volatile int* 
   atomicOr(p.status, kDevWaitTimeout);
 }
 
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u. The quick division is within 2 ulp and gives 0 for a divisor past
+// 2^126, where the quotient is below 2^-118 for any g that has one.
+__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-// Barrier of the four epilogue warps that also ands their predicates.
+// Barrier of a kernel's epilogue warps that also ands their predicates.
+template <int EPILOGUE_THREADS>
 __device__ __forceinline__ bool epilogue_all(bool ok) {
   uint32_t all;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(all)
-      : "r"(ok ? 1u : 0u)
+      : "r"(ok ? 1u : 0u), "n"(EPILOGUE_THREADS)
       : "memory");
   return all != 0;
 }
@@ -126,13 +130,17 @@ struct Lanes {
   static constexpr int PER_SM = BN <= 128 ? 2 : 1;
   static constexpr int STAGES = (PER_SM == 2 ? 104 * 1024 : 196 * 1024) / STAGE;
   static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
+  // Epilogue warps, one or two for each quarter of the lanes (1024 x 1024,
+  // k 1024: 256 tokens to a tile 9.4 us with four, 8.0 with eight; 16 tokens
+  // 3.3 and 3.5).
+  static constexpr int WARPS = BN <= 32 ? 4 : 8, THREADS = 64 + 32 * WARPS;
   static constexpr uint32_t TURN = 8 * 32 * 4;  // store_turned's slice of a warp
-  static constexpr size_t SMEM = 1024 + STAGES * STAGE + 256 + BN * sizeof(float) + 4 * TURN;
+  static constexpr size_t SMEM = 1024 + STAGES * STAGE + 256 + BN * sizeof(float) + WARPS * TURN;
   static_assert(BN * LANES * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
 };
 
 template <typename OUT, int BN, bool GATED>
-__global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __grid_constant__ TcLinear p) {
+__global__ void __launch_bounds__(Lanes<BN>::THREADS, Lanes<BN>::PER_SM) linear_channels_kernel(const __grid_constant__ TcLinear p) {
   using L = Lanes<BN>;
   constexpr int STAGES = L::STAGES, CHANNELS = GATED ? LANES / 2 : LANES;
   extern __shared__ uint8_t smem_raw[];
@@ -148,7 +156,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   uint32_t rank, splits;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x / splits) * CHANNELS, t0 = static_cast<int64_t>(blockIdx.y) * BN;
+  // Clusters of one channel tile follow one another: they share its weights in L2.
+  const int64_t j0 = static_cast<int64_t>(blockIdx.y) * CHANNELS, t0 = static_cast<int64_t>(blockIdx.x / splits) * BN;
   const uint32_t kb0 = p.total_kb * rank / splits, kb1 = p.total_kb * (rank + 1) / splits;
 
   if (threadIdx.x == 0) {
@@ -240,15 +249,15 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
       (void)mbar_wait_bounded(done, 0);
     }
   } else {
-    // ---------------- epilogue (warps 2..5), first part ----------------
+    // ---------------- epilogue (the other warps), first part ----------------
     if (p.after_quantize) wait_previous_launch();
-    for (int c = threadIdx.x - 64; c < BN; c += 128) token_scale[c] = t0 + c < p.m ? p.a_scale[t0 + c] : 0.0f;
+    for (int c = threadIdx.x - 64; c < BN; c += 32 * L::WARPS) token_scale[c] = t0 + c < p.m ? p.a_scale[t0 + c] : 0.0f;
   }
 
   // A thread of the epilogue owns a channel: in the direct form (an ungated
   // tile of one block) its accumulator lane, else a lane of the joined sums,
   // where a gated tile has half as many and splits the tokens over its warps.
-  const int ew = warp & 3, cw = GATED ? ew & 1 : ew;
+  const int quarter = warp & 3, ew = (warp - 2) & (L::WARPS - 1), cw = GATED ? quarter & 1 : quarter;
   const int64_t w0 = j0 + cw * 32, j = w0 + lane;  // the warp's first channel, this thread's
   const int tokens = static_cast<int>(min(p.m - t0, static_cast<int64_t>(BN)));
   OUT* out = static_cast<OUT*>(p.out) + t0 * p.ld_out + w0;
@@ -271,11 +280,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   int4* sums = reinterpret_cast<int4*>(smem);  // [BN / 4][LANES], once the stages are consumed
   if (warp >= 2) {
     if (!mbar_wait_bounded(done, 0) && !*abort_flag) report_timeout(p, abort_flag);
-    (void)epilogue_all(true);  // the token scales are in place
+    (void)epilogue_all<32 * L::WARPS>(true);  // the token scales are in place
     tc_fence_after();
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-    for (int c = 0; c < tokens; c += 32) {
+    for (int c = ew / 4 * 32; c < tokens; c += L::WARPS * 8) {
       uint32_t v[32];
       __syncwarp();
       tmem_ld_32x32b_x32(taddr + c, v);
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
         } else {
 #pragma unroll
           for (int e = i; e < i + 8; e += 4)
-            sums[((c + e) / 4) * LANES + ew * 32 + lane] =
+            sums[((c + e) / 4) * LANES + quarter * 32 + lane] =
                 make_int4(static_cast<int>(v[e]), static_cast<int>(v[e + 1]), static_cast<int>(v[e + 2]),
                           static_cast<int>(v[e + 3]));
         }
@@ -300,30 +309,38 @@ __global__ void __launch_bounds__(THREADS, 1) linear_channels_kernel(const __gri
   }
   if (!direct) {
     // Each block of the cluster joins a share of the tile's tokens, four at a
-    // time; all the blocks' parts of them are in flight together.
+    // time; all the blocks' parts of the next four are on their way meanwhile.
     cluster_sync();
     if (warp >= 2) {
-      constexpr int WARPS_PER_TOKEN = CHANNELS / 32, SHARES = 4 / WARPS_PER_TOKEN;
-      const int step = 4 * static_cast<int>(splits) * SHARES;
-      for (int c = 4 * (static_cast<int>(rank) * SHARES + ew / WARPS_PER_TOKEN); c < tokens; c += step) {
-        int4 part[GATED ? 2 : 1][kMaxSplits];
+      constexpr int WARPS_PER_TOKEN = CHANNELS / 32, SHARES = L::WARPS / WARPS_PER_TOKEN, PARTS = GATED ? 2 : 1;
+      const int share = GATED ? (ew / 4) * 2 + quarter / 2 : ew / 4, step = 4 * static_cast<int>(splits) * SHARES;
+      int4 next[PARTS][kMaxSplits];
+      auto fetch = [&](int c) {
 #pragma unroll
         for (int r = 0; r < kMaxSplits; ++r)
 #pragma unroll
-          for (int h = 0; h < (GATED ? 2 : 1); ++h)
-            part[h][r] = r < static_cast<int>(splits)
+          for (int h = 0; h < PARTS; ++h)
+            next[h][r] = r < static_cast<int>(splits)
                              ? ld_cluster(&sums[(c / 4) * LANES + h * CHANNELS + cw * 32 + lane], r)
                              : make_int4(0, 0, 0, 0);
+      };
+      int c = 4 * (static_cast<int>(rank) * SHARES + share);
+      if (c < tokens) fetch(c);
+      for (; c < tokens; c += step) {
+        int4 total[PARTS];
 #pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h)
+        for (int h = 0; h < PARTS; ++h) {
+          total[h] = next[h][0];
 #pragma unroll
           for (int r = 1; r < kMaxSplits; ++r) {
-            part[h][0].x += part[h][r].x;
-            part[h][0].y += part[h][r].y;
-            part[h][0].z += part[h][r].z;
-            part[h][0].w += part[h][r].w;
+            total[h].x += next[h][r].x;
+            total[h].y += next[h][r].y;
+            total[h].z += next[h][r].z;
+            total[h].w += next[h][r].w;
           }
-        const int4 a = part[0][0], u = part[GATED ? 1 : 0][0];
+        }
+        if (c + step < tokens) fetch(c + step);
+        const int4 a = total[0], u = total[PARTS - 1];
         const float y[4] = {value(c, a.x, u.x), value(c + 1, a.y, u.y), value(c + 2, a.z, u.z), value(c + 3, a.w, u.w)};
         store_turned<OUT, 4>(out + c * p.ld_out, p.ld_out, y, slice, lane, tokens - c, p.n - w0, p.vector_rows);
       }
@@ -492,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
       if (!ok && !*abort_flag) report_timeout(p, abort_flag);
       // The column values are in place, and the four warps stop together or
       // not at all: the next tile's barrier needs all of them.
-      if (!epilogue_all(ok)) break;
+      if (!epilogue_all<128>(ok)) break;
       tc_fence_after();
       OUT* orow = static_cast<OUT*>(p.out) + t * p.ld_out + n0;
       const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + acc * BN;
@@ -540,22 +557,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
 
 // ---- launches --------------------------------------------------------------------------
 template <typename Kernel>
-cudaError_t launch(Kernel kernel, std::atomic<uint64_t>& configured, dim3 grid, unsigned cluster, size_t smem,
-                   const TcLinear& p, cudaStream_t stream) {
+cudaError_t launch(Kernel kernel, std::atomic<uint64_t>& configured, dim3 grid, unsigned threads, unsigned cluster,
+                   size_t smem, const TcLinear& p, cudaStream_t stream) {
   const cudaError_t e = raise_smem_limit_once(kernel, static_cast<int>(smem), configured);
   if (e != cudaSuccess) return e;
-  return launch_chained(kernel, grid, THREADS, smem, cluster, stream, p);
+  return launch_chained(kernel, grid, threads, smem, cluster, stream, p);
 }
 
 template <typename OUT, int N, bool GATED>
 cudaError_t launch_channels(const TcLinear& p, dim3 grid, unsigned splits, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  return launch(linear_channels_kernel<OUT, N, GATED>, configured, grid, splits, Lanes<N>::SMEM, p, stream);
+  return launch(linear_channels_kernel<OUT, N, GATED>, configured, grid, Lanes<N>::THREADS, splits, Lanes<N>::SMEM, p,
+                stream);
 }
 template <typename OUT, bool GATED>
 cudaError_t launch_tokens(const TcLinear& p, unsigned grid, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  return launch(linear_tokens_kernel<OUT, GATED>, configured, dim3(grid), 1, TOKENS_SMEM, p, stream);
+  return launch(linear_tokens_kernel<OUT, GATED>, configured, dim3(grid), THREADS, 1, TOKENS_SMEM, p, stream);
 }
 
 template <typename F>
@@ -563,6 +581,53 @@ cudaError_t with_type(uint32_t type, F&& f) {
   if (type == RNS8_CUDA_TYPE_BF16) return f(__nv_bfloat16{});
   if (type == RNS8_CUDA_TYPE_F16) return f(__half{});
   return f(float{});
+}
+
+// Which form, tile and split a product runs, by an estimate of its time in us.
+// With spans of 128 bytes of k, a block streams one in 0.12 us + its bytes at
+// 155 GB/s when it has its SM to itself, at 75 GB/s beside another one; what a
+// tile costs besides grows with its tokens, more when blocks join their sums,
+// less the more of them share that; HBM gives the weights at 6.3 TB/s, less
+// when several token tiles ask for them or when one block an SM does. Blocks
+// that join wait for one another, so they are kept to one wave, with a tenth of
+// the SMs to spare (a cluster needs its blocks free in one place).
+// The constants are fitted to sweeps of both forms over 1 to 3000 tokens, 512
+// to 8192 channels and k. Some of them, in us, as tokens to a tile / blocks to a
+// cluster: 64 tokens 4096 x 4096: 8.4 as 64/4, 9.8 as 64/8, 12.0 as 16/1; 256
+// tokens: 11.7 as 64/2, 14.5 as 256/2, 17.3 tokens on lanes; 700 tokens 8192 x
+// 8192: 51.5 tokens on lanes, 57 as 128/1, 61 as 128/2.
+struct Choice {
+  bool tokens_on_lanes;
+  int tile;
+  unsigned splits;
+  double us;
+};
+Choice choose(int64_t m, int64_t n, int64_t total_kb, bool gated, int sm_count) {
+  const double weight_us = static_cast<double>(gated ? 2 * n : n) * total_kb * BK / 6.3e6;
+  const double sms = sm_count;
+  auto ceil_div = [](double a, double b) { return std::ceil(a / b); };
+  const double units = ceil_div(m, LANES) * ceil_div(n, gated ? BN / 2 : BN);
+  Choice best{true, 0, 1, 4.2 + std::max(weight_us, ceil_div(units, sms) * total_kb * 0.43)};
+  const double channel_tiles = ceil_div(n, gated ? LANES / 2 : LANES);
+  if (channel_tiles > 65535) return best;  // the grid's y extent
+  for (int tile = 16; tile <= 256; tile *= 2) {
+    const double token_tiles = ceil_div(m, tile), tiles = token_tiles * channel_tiles;
+    const int per_sm = tile <= 128 ? 2 : 1;
+    const double bytes = (LANES + tile) * BK * 1e-3, hbm = weight_us * (1 + 0.1 * (std::min(token_tiles, 5.0) - 1));
+    for (unsigned splits = 1; splits <= kMaxSplits && (splits == 1 || total_kb >= 2 * splits); splits *= 2) {
+      const double blocks = tiles * splits, waves = ceil_div(blocks, per_sm * sms);
+      const bool shared = per_sm == 2 && blocks > sms;
+      if (splits > 1 && blocks > 0.9 * per_sm * sms) break;
+      const double span = shared ? bytes / 75 : 0.12 + bytes / 155;
+      double rest = 0.1 + 0.011 * tile + 0.02 * tile / splits;
+      if (shared) rest = 1.6 * rest + (splits == kMaxSplits ? 1.5 : 0.0);
+      if (splits == 1 && !gated) rest = 0.005 * tile;
+      const double us = 2.9 + waves * rest + std::max(shared ? hbm : 1.07 * hbm, waves * ceil_div(total_kb, splits) * span);
+      if (us < best.us) best = Choice{false, tile, splits, us};
+    }
+    if (tile >= m) break;
+  }
+  return best;
 }
 
 }  // namespace
@@ -577,9 +642,11 @@ cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
   const size_t elem = a.out_type == RNS8_CUDA_TYPE_F32 ? 4 : 2;
   p.vector_rows = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ld_out * elem % 16 == 0;
   const int64_t w_rows = a.gated ? 2 * a.n : a.n;
-  const int cols = a.gated ? BN / 2 : BN;
-  const uint64_t m_tiles = (a.m + LANES - 1) / LANES, n_tiles = (a.n + cols - 1) / cols;
-  if (m_tiles * n_tiles >= static_cast<uint64_t>(sm_count) * 3 / 4) {
+  const Choice c = choose(a.m, a.n, p.total_kb, a.gated, sm_count);
+
+  if (c.tokens_on_lanes) {
+    const int cols = a.gated ? BN / 2 : BN;
+    const uint64_t m_tiles = (a.m + LANES - 1) / LANES, n_tiles = (a.n + cols - 1) / cols;
     if (m_tiles * n_tiles >= (1ull << 32)) return cudaErrorInvalidValue;
     if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, LANES) ||
         !encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, LANES))
@@ -594,27 +661,22 @@ cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
     });
   }
 
-  int tile = 16;
-  while (tile < 256 && tile < a.m) tile *= 2;
   const int channels = a.gated ? LANES / 2 : LANES;
   if (!encode_rows_i8(&p.tm_weights, a.w, w_rows, a.k, a.ld_w, static_cast<uint32_t>(channels)) ||
-      !encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, static_cast<uint32_t>(tile)))
+      !encode_rows_i8(&p.tm_tokens, a.a, a.m, a.k, a.ld_a, static_cast<uint32_t>(c.tile)))
     return cudaErrorInvalidValue;
-  const uint64_t token_tiles = (a.m + tile - 1) / tile, channel_tiles = (a.n + channels - 1) / channels;
-  const uint64_t tiles = token_tiles * channel_tiles, room = static_cast<uint64_t>(sm_count) * (tile <= 128 ? 2 : 1);
-  unsigned splits = 1;
-  while (splits < kMaxSplits && tiles * splits * 2 <= room && p.total_kb >= 4 * splits) splits *= 2;
-  const dim3 grid(static_cast<unsigned>(channel_tiles * splits), static_cast<unsigned>(token_tiles));
+  const dim3 grid(static_cast<unsigned>((a.m + c.tile - 1) / c.tile * c.splits),
+                  static_cast<unsigned>((a.n + channels - 1) / channels));
   return with_type(a.out_type, [&](auto t) {
     using OUT = decltype(t);
     auto go = [&](auto g) {
       constexpr bool G = decltype(g)::value;
-      switch (tile) {
-        case 16: return launch_channels<OUT, 16, G>(p, grid, splits, stream);
-        case 32: return launch_channels<OUT, 32, G>(p, grid, splits, stream);
-        case 64: return launch_channels<OUT, 64, G>(p, grid, splits, stream);
-        case 128: return launch_channels<OUT, 128, G>(p, grid, splits, stream);
-        default: return launch_channels<OUT, 256, G>(p, grid, splits, stream);
+      switch (c.tile) {
+        case 16: return launch_channels<OUT, 16, G>(p, grid, c.splits, stream);
+        case 32: return launch_channels<OUT, 32, G>(p, grid, c.splits, stream);
+        case 64: return launch_channels<OUT, 64, G>(p, grid, c.splits, stream);
+        case 128: return launch_channels<OUT, 128, G>(p, grid, c.splits, stream);
+        default: return launch_channels<OUT, 256, G>(p, grid, c.splits, stream);
       }
     };
     return a.gated ? go(std::true_type{}) : go(std::false_type{});

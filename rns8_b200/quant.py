@@ -64,24 +64,20 @@ def check_status(device: int = 0) -> None:
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """t as a 2-D tensor with contiguous rows."""
-    if t.dim() != 2:
-        if t.dim() == 0:
-            raise ValueError(f"{name}: expected at least one dimension")
-        t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    """t as a 2-D tensor (a view where one exists)."""
+    if t.dim() == 2:
+        return t
+    if t.dim() == 0:
+        raise ValueError(f"{name}: expected at least one dimension")
+    return t.reshape(-1, t.shape[-1])
+
+
+def _ld(t: torch.Tensor, name: str) -> int:
+    """Leading dimension of a 2-D tensor whose rows are contiguous."""
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{name}: elements of a row must be contiguous")
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _same_device(device: int, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"{name}: expected a tensor on cuda:{device}")
+    return ld if rows > 1 else max(cols, 1)
 
 
 def _float_type(t: torch.Tensor, name: str) -> int:
@@ -98,6 +94,15 @@ def _cuda_device(t: torch.Tensor, name: str) -> int:
     return device
 
 
+def _vector(t: torch.Tensor, size: int, device: int, name: str) -> int:
+    """Address of a 32-bit vector."""
+    if t.dtype != torch.float32 or t.shape != (size,) or not t.is_contiguous():
+        raise TypeError(f"{name}: expected a contiguous float32 vector of {size}")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a tensor on cuda:{device}")
+    return t.data_ptr()
+
+
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) with x ~ q * scale[..., None]: int8 rows and one 32-bit scale
     per row. Rows of q start on 16-byte boundaries (its leading dimension is
@@ -110,32 +115,36 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if cols == 0:
         raise ValueError("x: rows are empty")
     ld = (cols + 15) // 16 * 16
-    q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    desc = QUANTIZE_DESC.pack(QUANTIZE_DESC.size, 1, 0, device, code, rows, cols, _ld(x), ld, x.data_ptr(), q.data_ptr(),
-                              scale.data_ptr(), _stream(device))
-    check(lib().rns8_cuda_quantize_rows_device(desc), "rns8_cuda_quantize_rows_device")
+    q = x.new_empty((rows, ld), dtype=torch.int8)
+    scale = x.new_empty(rows, dtype=torch.float32)
+    desc = QUANTIZE_DESC.pack(QUANTIZE_DESC.size, 1, 0, device, code, rows, cols, _ld(x, "x"), ld, x.data_ptr(),
+                              q.data_ptr(), scale.data_ptr(), _stream(device))
+    status = lib().rns8_cuda_quantize_rows_device(desc)
+    if status:
+        check(status, "rns8_cuda_quantize_rows_device")
+    if ld != cols:
+        q = q[:, :cols]
+    if len(shape) == 2:
+        return q, scale
     if len(shape) == 1:
-        return q[0, :cols], scale[0]
-    return q[:, :cols].unflatten(0, shape[:-1]) if len(shape) > 2 else q[:, :cols], scale.view(shape[:-1])
+        return q[0], scale[0]
+    return q.unflatten(0, shape[:-1]), scale.view(shape[:-1])
 
 
-@functools.lru_cache(maxsize=1024)
-def _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, ld_out, align_a, align_w, has_bias):
+@functools.lru_cache(maxsize=4096)
+def _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, align_a, align_w):
     # Pointers stand for their alignments only: the query reads no memory.
-    desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, ld_out,
-                            4096 + align_a, 4096 if a_type == _I8 else 0, 4096 + align_w, 4096, 4096 * has_bias, 4096, 0,
-                            0, 0, 0)
+    desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, n,
+                            4096 + align_a, 4096 if a_type == _I8 else 0, 4096 + align_w, 4096, 0, 4096, 0, 0, 0, 0)
     return lib().rns8_cuda_linear_scratch_bytes(desc)
 
 
-def _linear(a, a_type, a_scale, w, w_scale, bias, gated, out_dtype):
-    device = _cuda_device(a, "activations")
+def _linear(a, a_type, a_scale, device, w, w_scale, bias, gated, out_dtype):
     lead = a.shape[:-1]
-    a = _rows(a, "activations")
+    if len(lead) != 1:
+        a = _rows(a, "activations")
     if w.dtype != torch.int8 or w.dim() != 2:
         raise TypeError("w: expected a 2-D int8 tensor (output channels x inputs)")
-    w = _rows(w, "w")
     m, k = a.shape
     rows, wk = w.shape
     if wk != k:
@@ -145,27 +154,25 @@ def _linear(a, a_type, a_scale, w, w_scale, bias, gated, out_dtype):
     n = rows // 2 if gated else rows
     if n == 0 or k == 0:
         raise ValueError("w: empty")
-    if w_scale.dtype != torch.float32 or w_scale.shape != (rows,) or not w_scale.is_contiguous():
-        raise TypeError(f"w_scale: expected a contiguous float32 vector of {rows}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (rows,) or not bias.is_contiguous()):
-        raise TypeError(f"bias: expected a contiguous float32 vector of {rows}")
-    _same_device(device, w=w, w_scale=w_scale, bias=bias)
+    if w.get_device() != device:
+        raise ValueError(f"w: expected a tensor on cuda:{device}")
+    p_scale = _vector(w_scale, rows, device, "w_scale")
+    p_bias = _vector(bias, rows, device, "bias") if bias is not None else 0
     out_type = _TYPES.get(out_dtype)
     if out_type is None:
         raise TypeError(f"out_dtype: expected bfloat16, float16 or float32, got {out_dtype}")
-    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    out = a.new_empty((m, n), dtype=out_dtype)
     if m:
         flags = _GATED if gated else 0
-        ld_a, ld_w, pa, pw = _ld(a), _ld(w), a.data_ptr(), w.data_ptr()
-        need = _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, n, pa & 15, pw & 15,
-                               bias is not None)
-        scratch = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+        ld_a, ld_w, pa, pw = _ld(a, "activations"), _ld(w, "w"), a.data_ptr(), w.data_ptr()
+        need = _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, pa & 15, pw & 15)
+        scratch = a.new_empty(need, dtype=torch.uint8) if need else None
         desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, n, pa,
-                                a_scale.data_ptr() if a_scale is not None else 0, pw, w_scale.data_ptr(),
-                                bias.data_ptr() if bias is not None else 0, out.data_ptr(),
-                                scratch.data_ptr() if need else 0, need, device_status(device).data_ptr(),
-                                _stream(device))
-        check(lib().rns8_cuda_linear_device(desc), "rns8_cuda_linear_device")
+                                a_scale, pw, p_scale, p_bias, out.data_ptr(), scratch.data_ptr() if need else 0, need,
+                                device_status(device).data_ptr(), _stream(device))
+        status = lib().rns8_cuda_linear_device(desc)
+        if status:
+            check(status, "rns8_cuda_linear_device")
     return out if len(lead) == 1 else out.view(*lead, n)
 
 
@@ -179,83 +186,104 @@ def gemm_scaled(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise TypeError(f"a: expected int8, got {a.dtype}")
     if a_scale.dtype != torch.float32 or a_scale.shape != a.shape[:-1] or not a_scale.is_contiguous():
         raise TypeError("a_scale: expected a contiguous float32 tensor with one value per row of a")
-    if a_scale.get_device() != a.get_device():
+    device = _cuda_device(a, "a")
+    if a_scale.get_device() != device:
         raise ValueError("a_scale: expected a tensor on a's device")
-    return _linear(a, _I8, a_scale, w, w_scale, bias, gated, out_dtype)
+    return _linear(a, _I8, a_scale.data_ptr(), device, w, w_scale, bias, gated, out_dtype)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
            gated: bool = False, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """gemm_scaled(*quantize_rows(x), w, w_scale) in one call; the result has
     x's type unless out_dtype is given."""
-    return _linear(x, _float_type(x, "x"), None, w, w_scale, bias, gated, out_dtype or x.dtype)
+    code = _float_type(x, "x")
+    return _linear(x, code, 0, _cuda_device(x, "x"), w, w_scale, bias, gated, out_dtype or x.dtype)
 
 
-class _NormArgs:
-    """Checked arguments shared by the forward and backward calls."""
+def _norm_weights(x, device, tokens, dim, post_weight, pre_weight, gate):
+    """(weight type, groups, gate's leading dimension, post, pre, gate addresses)
+    of a norm's checked parameters."""
+    dtype, post, pre, p_gate, groups, ld_gate = None, 0, 0, 0, 1, dim
+    if post_weight is not None:
+        dtype, post = post_weight.dtype, post_weight.data_ptr()
+        if post_weight.shape != (dim,) or not post_weight.is_contiguous() or post_weight.get_device() != device:
+            raise ValueError(f"post_weight: expected a contiguous vector of {dim} on cuda:{device}")
+    if pre_weight is not None:
+        pre = pre_weight.data_ptr()
+        if pre_weight.shape != (dim,) or not pre_weight.is_contiguous() or pre_weight.get_device() != device:
+            raise ValueError(f"pre_weight: expected a contiguous vector of {dim} on cuda:{device}")
+        if dtype is not None and pre_weight.dtype != dtype:
+            raise TypeError("pre_weight: the weights and the gate share one type")
+        dtype = pre_weight.dtype
+    if gate is not None:
+        groups, gate_dim = gate.shape
+        if gate_dim != dim or gate.get_device() != device:
+            raise ValueError(f"gate: expected rows of {dim} on cuda:{device}")
+        if dtype is not None and gate.dtype != dtype:
+            raise TypeError("gate: the weights and the gate share one type")
+        if tokens and (groups == 0 or tokens % groups):
+            raise ValueError(f"gate: {groups} rows do not divide {tokens} tokens")
+        dtype, ld_gate, p_gate = gate.dtype, _ld(gate, "gate"), gate.data_ptr()
+    if dtype is None:
+        dtype = x.dtype
+    elif dtype != x.dtype and dtype != torch.float32:
+        raise TypeError(f"weights: expected {x.dtype} or float32, got {dtype}")
+    return _TYPES[dtype], groups, ld_gate, post, pre, p_gate
 
-    __slots__ = ("device", "code", "wcode", "tokens", "dim", "groups", "ld_gate", "post", "pre", "gate")
 
-    def __init__(self, x, y, post_weight, pre_weight, gate):
-        self.code = _float_type(x, "x")
-        self.device = device = _cuda_device(x, "x")
-        if y.dtype != x.dtype or y.shape != x.shape:
-            raise ValueError("y: expected x's type and shape")
-        self.tokens, self.dim = x.shape
-        if not 0 < self.dim <= MAX_DIM:
-            raise ValueError(f"x: rows must have 1 to {MAX_DIM} elements")
-        wdtype = None
-        for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-            if w is None:
-                continue
-            if w.shape != (self.dim,) or not w.is_contiguous():
-                raise ValueError(f"{name}: expected a contiguous vector of {self.dim}")
-            if wdtype is not None and w.dtype != wdtype:
-                raise TypeError(f"{name}: the weights and the gate share one type")
-            wdtype = w.dtype
-        self.groups, self.ld_gate, self.gate = 1, self.dim, 0
-        if gate is not None:
-            if gate.shape[1] != self.dim:
-                raise ValueError(f"gate: expected rows of {self.dim}")
-            if wdtype is not None and gate.dtype != wdtype:
-                raise TypeError("gate: the weights and the gate share one type")
-            wdtype = gate.dtype
-            self.groups = gate.shape[0]
-            if self.tokens and (self.groups == 0 or self.tokens % self.groups):
-                raise ValueError(f"gate: {self.groups} rows do not divide {self.tokens} tokens")
-            self.ld_gate, self.gate = _ld(gate), gate.data_ptr()
-        if wdtype is not None and wdtype not in (x.dtype, torch.float32):
-            raise TypeError(f"weights: expected {x.dtype} or float32, got {wdtype}")
-        self.wcode = self.code if wdtype is None else _TYPES[wdtype]
-        _same_device(device, y=y, post_weight=post_weight, pre_weight=pre_weight, gate=gate)
-        self.post = post_weight.data_ptr() if post_weight is not None else 0
-        self.pre = pre_weight.data_ptr() if pre_weight is not None else 0
+def _norm_rows(x, y, name):
+    """Type, device, sizes and 2-D forms of a norm's two activations."""
+    code = _float_type(x, name)
+    device = _cuda_device(x, name)
+    if y.shape != x.shape or y.dtype != x.dtype:
+        raise ValueError(f"y: expected {name}'s type and shape")
+    if y.get_device() != device:
+        raise ValueError(f"y: expected a tensor on cuda:{device}")
+    x, y = _rows(x, name), _rows(y, "y")
+    tokens, dim = x.shape
+    if not 0 < dim <= MAX_DIM:
+        raise ValueError(f"{name}: rows must have 1 to {MAX_DIM} elements")
+    return code, device, tokens, dim, x, y
 
 
 def _norm_forward(x, y, post_weight, pre_weight, gate, scale, eps, weight_offset, want_h, want_q):
     shape = x.shape
-    if y.shape != shape:
-        raise ValueError("y: expected x's shape")
-    x, y = _rows(x, "x"), _rows(y, "y")
-    gate = _rows(gate, "gate") if gate is not None else None
-    a = _NormArgs(x, y, post_weight, pre_weight, gate)
-    x_out = torch.empty((a.tokens, a.dim), dtype=x.dtype, device=x.device)
-    h = torch.empty((a.tokens, a.dim), dtype=x.dtype, device=x.device) if want_h else None
-    ld_q = (a.dim + 15) // 16 * 16
-    q = torch.empty((a.tokens, ld_q), dtype=torch.int8, device=x.device) if want_q else None
-    s = torch.empty(a.tokens, dtype=torch.float32, device=x.device) if want_q else None
-    if a.tokens:
-        desc = NORM_DESC.pack(NORM_DESC.size, 1, 0, a.device, a.code, a.wcode, scale, eps, weight_offset, a.tokens, a.dim,
-                              a.groups, _ld(x), _ld(y), a.ld_gate, a.dim, a.dim, ld_q, x.data_ptr(), y.data_ptr(),
-                              a.post, a.pre, a.gate, x_out.data_ptr(), h.data_ptr() if want_h else 0,
-                              q.data_ptr() if want_q else 0, s.data_ptr() if want_q else 0, _stream(a.device))
-        check(lib().rns8_cuda_residual_norm_device(desc), "rns8_cuda_residual_norm_device")
+    code, device, tokens, dim, x, y = _norm_rows(x, y, "x")
+    if gate is not None:
+        gate = _rows(gate, "gate")
+    wcode, groups, ld_gate, post, pre, p_gate = _norm_weights(x, device, tokens, dim, post_weight, pre_weight, gate)
+    x_out = x.new_empty((tokens, dim))
+    h = x.new_empty((tokens, dim)) if want_h else None
+    ld_q, q, s = (dim + 15) // 16 * 16, None, None
+    if want_q:
+        q = x.new_empty((tokens, ld_q), dtype=torch.int8)
+        s = x.new_empty(tokens, dtype=torch.float32)
+    if tokens:
+        desc = NORM_DESC.pack(NORM_DESC.size, 1, 0, device, code, wcode, scale, eps, weight_offset, tokens, dim, groups,
+                              _ld(x, "x"), _ld(y, "y"), ld_gate, dim, dim, ld_q, x.data_ptr(), y.data_ptr(), post, pre,
+                              p_gate, x_out.data_ptr(), h.data_ptr() if want_h else 0, q.data_ptr() if want_q else 0,
+                              s.data_ptr() if want_q else 0, _stream(device))
+        status = lib().rns8_cuda_residual_norm_device(desc)
+        if status:
+            check(status, "rns8_cuda_residual_norm_device")
+    if want_q and ld_q != dim:
+        q = q[:, :dim]
     if len(shape) == 2:
-        return x_out, h, q[:, :a.dim] if want_q else None, s
+        return x_out, h, q, s
     lead = shape[:-1]
-    return (x_out.view(shape), h.view(shape) if want_h else None,
-            (q[0, :a.dim] if len(lead) == 0 else q[:, :a.dim].unflatten(0, lead)) if want_q else None,
-            s.view(lead) if want_q else None)
+    if want_q:
+        q = q.unflatten(0, lead) if lead else q[0]
+        s = s.view(lead)
+    return x_out.view(shape), h.view(shape) if want_h else None, q, s
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_scratch(device, code, wcode, tokens, dim, groups, post, pre, gate):
+    # Sizes and which gradients are wanted decide: the query reads no memory.
+    desc = NORM_BACKWARD_DESC.pack(NORM_BACKWARD_DESC.size, 1, 0, device, code, wcode, 1.0, 1.0, 0.0, tokens, dim, groups,
+                                   *(dim,) * 8, 4096, 4096, 4096, 4096, 4096 * post, 4096 * pre, 4096 * gate, 4096, 4096,
+                                   4096 * post, 4096 * pre, 4096 * gate, 0, 0, 0)
+    return lib().rns8_cuda_residual_norm_backward_scratch_bytes(desc)
 
 
 def residual_norm_backward(d_x_out: torch.Tensor | None, d_h: torch.Tensor | None, x_out: torch.Tensor, y: torch.Tensor, *,
@@ -268,42 +296,48 @@ def residual_norm_backward(d_x_out: torch.Tensor | None, d_h: torch.Tensor | Non
     per token. Entries without their input are None."""
     shape = x_out.shape
     gate_shape = gate.shape if gate is not None else None
-    x_out, y = _rows(x_out, "x_out"), _rows(y, "y")
-    gate = _rows(gate, "gate") if gate is not None else None
-    a = _NormArgs(x_out, y, post_weight, pre_weight, gate)
-    grads = []
-    for name, g in (("d_x_out", d_x_out), ("d_h", d_h)):
-        if g is not None:
-            if g.shape != shape or g.dtype != x_out.dtype:
-                raise ValueError(f"{name}: expected x_out's type and shape")
-            _same_device(a.device, **{name: g})
-            g = _rows(g, name)
-        grads.append(g)
-    dxo, dh = grads
-    dev, t, dim = x_out.device, a.tokens, a.dim
-    d_x = torch.empty((t, dim), dtype=x_out.dtype, device=dev)
-    d_y = torch.empty((t, dim), dtype=x_out.dtype, device=dev)
-    d_post = torch.empty(dim, dtype=torch.float32, device=dev) if post_weight is not None else None
-    d_pre = torch.empty(dim, dtype=torch.float32, device=dev) if pre_weight is not None else None
-    d_gate = None
+    code, device, tokens, dim, x_out, y = _norm_rows(x_out, y, "x_out")
     if gate is not None:
-        d_gate = torch.empty((a.groups, dim), dtype=x_out.dtype if a.groups == t else torch.float32, device=dev)
-
-    def pack(scratch, size):
-        return NORM_BACKWARD_DESC.pack(
-            NORM_BACKWARD_DESC.size, 1, 0, a.device, a.code, a.wcode, scale, eps, weight_offset, t, dim, a.groups,
-            _ld(dxo) if dxo is not None else dim, _ld(dh) if dh is not None else dim, _ld(x_out), _ld(y), a.ld_gate, dim,
-            dim, dim, dxo.data_ptr() if dxo is not None else 0, dh.data_ptr() if dh is not None else 0,
-            x_out.data_ptr(), y.data_ptr(), a.post, a.pre, a.gate, d_x.data_ptr(), d_y.data_ptr(),
-            d_post.data_ptr() if d_post is not None else 0, d_pre.data_ptr() if d_pre is not None else 0,
-            d_gate.data_ptr() if d_gate is not None else 0, scratch, size, _stream(a.device))
-
-    handle = lib()
-    need = handle.rns8_cuda_residual_norm_backward_scratch_bytes(pack(0, 0))
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(handle.rns8_cuda_residual_norm_backward_device(pack(scratch.data_ptr() if need else 0, need)),
-          "rns8_cuda_residual_norm_backward_device")
-    return (d_x.view(shape), d_y.view(shape), d_post, d_pre, d_gate.view(gate_shape) if gate is not None else None)
+        gate = _rows(gate, "gate")
+    wcode, groups, ld_gate, post, pre, p_gate = _norm_weights(x_out, device, tokens, dim, post_weight, pre_weight, gate)
+    p_dxo = p_dh = 0
+    ld_dxo = ld_dh = dim
+    if d_x_out is not None:
+        if d_x_out.shape != shape or d_x_out.dtype != x_out.dtype or d_x_out.get_device() != device:
+            raise ValueError("d_x_out: expected x_out's type, shape and device")
+        d_x_out = _rows(d_x_out, "d_x_out")
+        p_dxo, ld_dxo = d_x_out.data_ptr(), _ld(d_x_out, "d_x_out")
+    if d_h is not None:
+        if d_h.shape != shape or d_h.dtype != x_out.dtype or d_h.get_device() != device:
+            raise ValueError("d_h: expected x_out's type, shape and device")
+        d_h = _rows(d_h, "d_h")
+        p_dh, ld_dh = d_h.data_ptr(), _ld(d_h, "d_h")
+    d_x = x_out.new_empty((tokens, dim))
+    d_y = x_out.new_empty((tokens, dim))
+    d_post = d_pre = d_gate = None
+    if post and pre:
+        d_post, d_pre = x_out.new_empty((2, dim), dtype=torch.float32).unbind(0)
+    elif post:
+        d_post = x_out.new_empty(dim, dtype=torch.float32)
+    elif pre:
+        d_pre = x_out.new_empty(dim, dtype=torch.float32)
+    if gate is not None:
+        d_gate = x_out.new_empty((groups, dim), dtype=x_out.dtype if groups == tokens else torch.float32)
+    need = _backward_scratch(device, code, wcode, tokens, dim, groups, post != 0, pre != 0, gate is not None)
+    scratch = x_out.new_empty(need, dtype=torch.uint8) if need else None
+    desc = NORM_BACKWARD_DESC.pack(
+        NORM_BACKWARD_DESC.size, 1, 0, device, code, wcode, scale, eps, weight_offset, tokens, dim, groups, ld_dxo, ld_dh,
+        _ld(x_out, "x_out"), _ld(y, "y"), ld_gate, dim, dim, dim, p_dxo, p_dh, x_out.data_ptr(), y.data_ptr(), post, pre,
+        p_gate, d_x.data_ptr(), d_y.data_ptr(), d_post.data_ptr() if post else 0, d_pre.data_ptr() if pre else 0,
+        d_gate.data_ptr() if gate is not None else 0, scratch.data_ptr() if need else 0, need, _stream(device))
+    status = lib().rns8_cuda_residual_norm_backward_device(desc)
+    if status:
+        check(status, "rns8_cuda_residual_norm_backward_device")
+    if len(shape) != 2:
+        d_x, d_y = d_x.view(shape), d_y.view(shape)
+    if gate is not None and len(gate_shape) != 2:
+        d_gate = d_gate.view(gate_shape)
+    return d_x, d_y, d_post, d_pre, d_gate
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -340,10 +374,11 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor
     (post_weight for y, pre_weight for h). Without post_weight y enters as it
     is; without pre_weight h is None. gate is one row of channels or rows that
     each serve an equal run of tokens. Gradients flow to every tensor."""
-    tensors = (x, y, post_weight, pre_weight, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _ResidualNorm.apply(*tensors, scale, eps, weight_offset)
-    return _norm_forward(*tensors, scale, eps, weight_offset, pre_weight is not None, False)[:2]
+    if torch.is_grad_enabled():
+        tensors = (x, y, post_weight, pre_weight, gate)
+        if any([t is not None and t.requires_grad for t in tensors]):
+            return _ResidualNorm.apply(*tensors, scale, eps, weight_offset)
+    return _norm_forward(x, y, post_weight, pre_weight, gate, scale, eps, weight_offset, pre_weight is not None, False)[:2]
 
 
 def residual_norm_quantized(x: torch.Tensor, y: torch.Tensor, *, pre_weight: torch.Tensor,
