@@ -64,7 +64,10 @@ RNS8_API rns8_status rns8_cuda_quantize_rows_device(const rns8_cuda_quantize_des
  *   acc[i][j] = sum over k of q[i][k] * w[j][k]          (exact, 32-bit)
  *   y[i][j]   = acc[i][j] * a_scale[i] * w_scale[j] + bias[j]
  * out = y rounded once to out_type. With RNS8_CUDA_LINEAR_GATED w holds 2n
- * rows, the first n the gate's: out = silu(y[i][j]) * y[i][n + j].
+ * rows, the first n the gate's: out = silu(y[i][j]) * y[i][n + j]. With out_type
+ * I8 the result comes as int8 rows with their scales in out_scale, quantised as
+ * above from its 32-bit values: the tokens of a next product, whose error then
+ * holds no rounding to a 16-bit type in between.
  * a is either int8 rows with their scales (a_type I8) or floating rows that
  * the call quantises as rns8_cuda_quantize_rows_device does (a_scale NULL).
  * w is n (2n) rows of k int8, as a checkpoint keeps a layer's output channels.
@@ -87,6 +90,7 @@ typedef struct rns8_cuda_linear_desc {
   const float* w_scale; /* [n], gated [2n] */
   const float* bias;    /* [n], gated [2n], or NULL */
   void* out;
+  float* out_scale; /* [m] with out_type I8, else NULL */
   void* scratch;
   uint64_t scratch_bytes;
   uint32_t* status;

@@ -46,7 +46,7 @@ rns8_status launch_result(cudaError_t e) {
 
 rns8_status check_linear(const rns8_cuda_linear_desc* d) {
   if (!valid_header(d) || (d->flags & ~RNS8_CUDA_LINEAR_GATED) || d->reserved) return RNS8_INVALID_ARGUMENT;
-  if (d->a_type > RNS8_CUDA_TYPE_I8 || !float_type(d->out_type)) return RNS8_INVALID_ARGUMENT;
+  if (d->a_type > RNS8_CUDA_TYPE_I8 || d->out_type > RNS8_CUDA_TYPE_I8) return RNS8_INVALID_ARGUMENT;
   if (d->m < 0 || d->n < 1 || d->k < 1 || d->m > kMaxExtent || d->n > kMaxExtent / 2 || d->k > kMaxExtent)
     return RNS8_INVALID_ARGUMENT;
   const int64_t w_rows = (d->flags & RNS8_CUDA_LINEAR_GATED) ? 2 * d->n : d->n;
@@ -57,6 +57,8 @@ rns8_status check_linear(const rns8_cuda_linear_desc* d) {
     if (d->m > 0 || d->a_type != RNS8_CUDA_TYPE_I8) return RNS8_INVALID_ARGUMENT;
   if (d->m > 0 && (!valid_rows(d->a, d->m, d->k, d->ld_a, type_size(d->a_type)) ||
                    !valid_rows(d->out, d->m, d->n, d->ld_out, type_size(d->out_type))))
+    return RNS8_INVALID_ARGUMENT;
+  if (!aligned_to(d->out_scale, 4) || (d->m > 0 && (d->out_type == RNS8_CUDA_TYPE_I8) != (d->out_scale != nullptr)))
     return RNS8_INVALID_ARGUMENT;
   return d->k > RNS8_CUDA_LINEAR_MAX_K ? RNS8_ACCUMULATION_OVERFLOW_RISK : RNS8_SUCCESS;
 }

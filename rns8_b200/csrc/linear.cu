@@ -52,11 +52,11 @@ cudaError_t align_rows(const int8_t* src, int64_t rows, int64_t cols, int64_t ld
   return launch_chained(align_rows_kernel, dim3(grid), 256, 0, 1, stream, src, rows, cols, ld, dst, ld_dst);
 }
 
-// What a call needs before its product, and where in scratch.
+// What a call needs around its product, and where in scratch.
 struct Steps {
-  bool align_w, align_a, quantize;
+  bool align_w, align_a, quantize, quantize_out;
   int64_t w_rows, ld;
-  uint64_t at_a, at_scale, bytes;
+  uint64_t at_a, at_scale, at_out, bytes;
 };
 Steps plan(const rns8_cuda_linear_desc& d) {
   Steps s{};
@@ -70,6 +70,9 @@ Steps plan(const rns8_cuda_linear_desc& d) {
   if (s.quantize || s.align_a) s.bytes += round_up(static_cast<uint64_t>(d.m) * s.ld, 256);
   s.at_scale = s.bytes;
   if (s.quantize) s.bytes += round_up(4ull * d.m, 256);
+  s.at_out = s.bytes;
+  s.quantize_out = d.out_type == RNS8_CUDA_TYPE_I8;
+  if (s.quantize_out) s.bytes += 4ull * static_cast<uint64_t>(d.m) * round_up(d.n, 4);
   if (s.bytes) s.bytes += 256;  // the caller's scratch may start anywhere
   return s;
 }
@@ -103,7 +106,14 @@ cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t st
     p.a = q;
     p.ld_a = s.ld;
   }
-  return linear_tc(p, sm_count, stream);
+  if (!s.quantize_out) return linear_tc(p, sm_count, stream);
+  p.out = scratch + s.at_out;
+  p.out_type = RNS8_CUDA_TYPE_F32;
+  p.ld_out = static_cast<int64_t>(round_up(d.n, 4));
+  e = linear_tc(p, sm_count, stream);
+  if (e != cudaSuccess) return e;
+  return quantize_rows(p.out, RNS8_CUDA_TYPE_F32, d.m, d.n, p.ld_out, static_cast<int8_t*>(d.out), d.ld_out, d.out_scale,
+                       stream);
 }
 
 }  // namespace rns8cuda

@@ -1,7 +1,8 @@
 """8-bit operators of large language models on torch CUDA tensors.
 
     quantize_rows            rows of activations or weights -> int8 rows + scales
-    gemm_scaled              int8 rows x int8 weights -> float, a scale per row and per output channel
+    gemm_scaled              int8 rows x int8 weights, a scale per row and per output channel -> float, or
+                             int8 rows again for the next product
     linear                   the same from float activations, quantised per row in the call
     residual_norm            x' = x + scale * gate * N(y) and h = N(x'), differentiable
     residual_norm_quantized  the same with h as int8 rows + scales, ready for gemm_scaled
@@ -20,6 +21,7 @@ from __future__ import annotations
 
 import functools
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -35,12 +37,24 @@ MAX_DIM = 32768
 # The descriptors of include/rns8/rns8_quant.h, packed field by field (a test
 # compares them with the C compiler's layout).
 QUANTIZE_DESC = struct.Struct("=QIIiI4q4Q")
-LINEAR_DESC = struct.Struct("=QIIiIII6q10Q")
+LINEAR_DESC = struct.Struct("=QIIiIII6q11Q")
 NORM_DESC = struct.Struct("=QIIiIIfff9q10Q")
 NORM_BACKWARD_DESC = struct.Struct("=QIIiIIfff11q15Q")
 
 _stream = torch._C._cuda_getCurrentRawStream
 _status: dict[int, torch.Tensor] = {}
+
+
+class QuantizedRows(NamedTuple):
+    """Activations as int8 rows with a 32-bit scale each, and the type that the
+    next product answers in."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    dtype: torch.dtype
+
+    def dequantize(self) -> torch.Tensor:
+        return (self.q.float() * self.scale[..., None]).to(self.dtype)
 
 
 def device_status(device: int = 0) -> torch.Tensor:
@@ -135,11 +149,12 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, align_a, align_w):
     # Pointers stand for their alignments only: the query reads no memory.
     desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, n,
-                            4096 + align_a, 4096 if a_type == _I8 else 0, 4096 + align_w, 4096, 0, 4096, 0, 0, 0, 0)
+                            4096 + align_a, 4096 if a_type == _I8 else 0, 4096 + align_w, 4096, 0, 4096,
+                            4096 if out_type == _I8 else 0, 0, 0, 0, 0)
     return lib().rns8_cuda_linear_scratch_bytes(desc)
 
 
-def _linear(a, a_type, a_scale, device, w, w_scale, bias, gated, out_dtype):
+def _linear(a, a_type, a_scale, device, w, w_scale, bias, gated, out_dtype, quantize):
     lead = a.shape[:-1]
     if len(lead) != 1:
         a = _rows(a, "activations")
@@ -161,27 +176,46 @@ def _linear(a, a_type, a_scale, device, w, w_scale, bias, gated, out_dtype):
     out_type = _TYPES.get(out_dtype)
     if out_type is None:
         raise TypeError(f"out_dtype: expected bfloat16, float16 or float32, got {out_dtype}")
-    out = a.new_empty((m, n), dtype=out_dtype)
+    out_scale, ld_out, p_out_scale = None, n, 0
+    if quantize:
+        out_type, ld_out = _I8, (n + 15) // 16 * 16
+        out = a.new_empty((m, ld_out), dtype=torch.int8)
+        out_scale = a.new_empty(m, dtype=torch.float32)
+        p_out_scale = out_scale.data_ptr()
+    else:
+        out = a.new_empty((m, n), dtype=out_dtype)
     if m:
         flags = _GATED if gated else 0
         ld_a, ld_w, pa, pw = _ld(a, "activations"), _ld(w, "w"), a.data_ptr(), w.data_ptr()
         need = _linear_scratch(device, flags, a_type, out_type, m, n, k, ld_a, ld_w, pa & 15, pw & 15)
         scratch = a.new_empty(need, dtype=torch.uint8) if need else None
-        desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, n, pa,
-                                a_scale, pw, p_scale, p_bias, out.data_ptr(), scratch.data_ptr() if need else 0, need,
-                                device_status(device).data_ptr(), _stream(device))
+        desc = LINEAR_DESC.pack(LINEAR_DESC.size, 1, flags, device, a_type, out_type, 0, m, n, k, ld_a, ld_w, ld_out, pa,
+                                a_scale, pw, p_scale, p_bias, out.data_ptr(), p_out_scale,
+                                scratch.data_ptr() if need else 0, need, device_status(device).data_ptr(),
+                                _stream(device))
         status = lib().rns8_cuda_linear_device(desc)
         if status:
             check(status, "rns8_cuda_linear_device")
+    if quantize:
+        if ld_out != n:
+            out = out[:, :n]
+        if len(lead) != 1:
+            out, out_scale = (out.unflatten(0, lead), out_scale.view(lead)) if lead else (out[0], out_scale[0])
+        return QuantizedRows(out, out_scale, out_dtype)
     return out if len(lead) == 1 else out.view(*lead, n)
 
 
 def gemm_scaled(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
-                bias: torch.Tensor | None = None, gated: bool = False,
-                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+                bias: torch.Tensor | None = None, gated: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+                quantize: bool | None = None):
     """(a @ w.T) * a_scale[..., None] * w_scale + bias from int8 a (tokens x k)
     and int8 w (output channels x k), summed exactly in 32-bit integers. With
-    gated, w's first half are the gate's channels: silu(first) * second."""
+    gated, w's first half are the gate's channels: silu(first) * second.
+
+    The result is a tensor of out_dtype, or, with quantize, QuantizedRows made
+    from the 32-bit values: int8 in, int8 out, for a chain of products. A gated
+    product's result is the next product's tokens, so there quantize is the
+    default; pass quantize=False for a tensor."""
     if a.dtype != torch.int8:
         raise TypeError(f"a: expected int8, got {a.dtype}")
     if a_scale.dtype != torch.float32 or a_scale.shape != a.shape[:-1] or not a_scale.is_contiguous():
@@ -189,15 +223,19 @@ def gemm_scaled(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale
     device = _cuda_device(a, "a")
     if a_scale.get_device() != device:
         raise ValueError("a_scale: expected a tensor on a's device")
-    return _linear(a, _I8, a_scale.data_ptr(), device, w, w_scale, bias, gated, out_dtype)
+    return _linear(a, _I8, a_scale.data_ptr(), device, w, w_scale, bias, gated, out_dtype,
+                   gated if quantize is None else quantize)
 
 
-def linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
-           gated: bool = False, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+def linear(x: torch.Tensor | QuantizedRows, w: torch.Tensor, w_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
+           gated: bool = False, out_dtype: torch.dtype | None = None, quantize: bool = False):
     """gemm_scaled(*quantize_rows(x), w, w_scale) in one call; the result has
-    x's type unless out_dtype is given."""
+    x's type unless out_dtype is given. QuantizedRows go in as they are."""
+    if isinstance(x, QuantizedRows):
+        return gemm_scaled(x.q, x.scale, w, w_scale, bias=bias, gated=gated, out_dtype=out_dtype or x.dtype,
+                           quantize=quantize)
     code = _float_type(x, "x")
-    return _linear(x, code, 0, _cuda_device(x, "x"), w, w_scale, bias, gated, out_dtype or x.dtype)
+    return _linear(x, code, 0, _cuda_device(x, "x"), w, w_scale, bias, gated, out_dtype or x.dtype, quantize)
 
 
 def _norm_weights(x, device, tokens, dim, post_weight, pre_weight, gate):

@@ -139,7 +139,7 @@ def test_gemm_scaled_shapes(quant, m, n, k, gated):
     elif dtype == torch.float16:
         s = s / k**0.5
     bias = b if (m + k) % 2 else None
-    got = quant.gemm_scaled(a, s, w, ws, bias=bias, gated=gated, out_dtype=dtype)
+    got = quant.gemm_scaled(a, s, w, ws, bias=bias, gated=gated, out_dtype=dtype, quantize=False)
     assert got.shape == (m, n) and got.dtype == dtype
     check_close(got, *linear_ref(a, s, w, ws, bias, gated), dtype)
 
@@ -183,8 +183,37 @@ def test_linear(quant, m, n, k, gated, dtype):
     assert got.dtype == dtype
     check_close(got, want, err, dtype)
     # The one call equals its two steps bit for bit.
-    two = quant.gemm_scaled(*quant.quantize_rows(x), w, ws, bias=b, gated=gated, out_dtype=dtype)
+    two = quant.gemm_scaled(*quant.quantize_rows(x), w, ws, bias=b, gated=gated, out_dtype=dtype, quantize=False)
     assert torch.equal(got, two)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 512, 1024), (3, 40, 77), (48, 300, 4096), (200, 1001, 520),
+                                   (1500, 768, 256)])
+def test_quantized_result(quant, m, n, k, gated):
+    """int8 rows out equal the quantisation, by its definition, of the 32-bit
+    result; linear takes them as they are and answers in their type."""
+    a, s, w, ws, b = operands(m, 2 * n if gated else n, k, m + n)
+    s = s / k**0.5
+    y = quant.gemm_scaled(a, s, w, ws, bias=b, gated=gated, out_dtype=torch.float32, quantize=False)
+    rows = quant.gemm_scaled(a, s, w, ws, bias=b, gated=gated, out_dtype=torch.float16, quantize=True)
+    q, scale = quantize_ref(y)
+    assert rows.dtype == torch.float16 and rows.q.shape == (m, n)
+    assert np.array_equal(rows.q.cpu().numpy(), q) and np.array_equal(rows.scale.cpu().numpy(), scale)
+    assert torch.allclose(rows.dequantize().float(), y, rtol=0, atol=float(y.abs().max()) / 200)
+    _, _, w2, ws2, _ = operands(1, 33, n, 3)
+    ws2 = ws2 / 10
+    out = quant.linear(rows, w2, ws2)
+    assert out.dtype == torch.float16
+    assert torch.equal(out, quant.gemm_scaled(rows.q, rows.scale, w2, ws2, out_dtype=torch.float16))
+    assert torch.equal(out, quant.linear(y, w2, ws2, out_dtype=torch.float16))
+    if gated:
+        again = quant.gemm_scaled(a, s, w, ws, bias=b, gated=True)
+        assert isinstance(again, quant.QuantizedRows) and again.dtype == torch.bfloat16 and torch.equal(again.q, rows.q)
+    x = torch.randn(2, m, k, device="cuda")
+    rows = quant.linear(x, w, ws, gated=gated, quantize=True)
+    assert rows.q.shape == (2, m, n) and rows.scale.shape == (2, m)
+    assert quant.linear(x[:, :0], w, ws, gated=gated, quantize=True).q.shape == (2, 0, n)
 
 
 @pytest.mark.parametrize("m", [1, 3, 8, 20, 200])
@@ -240,11 +269,11 @@ def test_output_leading_dimension_and_offsets_past_32_bits(quant):
     view_a.copy_(a)
     out = torch.zeros(2 * ld + n + 8, dtype=torch.bfloat16, device="cuda")
     args = [quant.LINEAR_DESC.size, 1, 0, 0, 3, 0, 0, m, n, k, ld, k, ld, view_a.data_ptr(), s.data_ptr(), w.data_ptr(),
-            ws.data_ptr(), b.data_ptr(), out.data_ptr(), 0, 0, quant.device_status(0).data_ptr(),
+            ws.data_ptr(), b.data_ptr(), out.data_ptr(), 0, 0, 0, quant.device_status(0).data_ptr(),
             torch.cuda.current_stream().cuda_stream]
     need = lib().rns8_cuda_linear_scratch_bytes(quant.LINEAR_DESC.pack(*args))
     scratch = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
-    args[19:21] = scratch.data_ptr(), need
+    args[20:22] = scratch.data_ptr(), need
     assert lib().rns8_cuda_linear_device(quant.LINEAR_DESC.pack(*args)) == 0
     got = torch.as_strided(out, (m, n), (ld, 1))
     check_close(got, *linear_ref(a, s, w, ws, b, False), torch.bfloat16)
@@ -260,11 +289,11 @@ def test_scratch_too_small_is_refused(quant, m):
     _, _, w, ws, _ = operands(1, 33, 35, 2)
     out = torch.zeros(m, 33, dtype=torch.bfloat16, device="cuda")
     args = [quant.LINEAR_DESC.size, 1, 0, 0, 0, 0, 0, m, 33, 35, 35, 35, 33, x.data_ptr(), 0, w.data_ptr(), ws.data_ptr(),
-            0, out.data_ptr(), 0, 0, quant.device_status(0).data_ptr(), 0]
+            0, out.data_ptr(), 0, 0, 0, quant.device_status(0).data_ptr(), 0]
     need = lib().rns8_cuda_linear_scratch_bytes(quant.LINEAR_DESC.pack(*args))
     if need:
         scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
-        args[19:21] = scratch.data_ptr(), need - 1
+        args[20:22] = scratch.data_ptr(), need - 1
         assert lib().rns8_cuda_linear_device(quant.LINEAR_DESC.pack(*args)) == 7
         assert int(torch.count_nonzero(out)) == 0
 

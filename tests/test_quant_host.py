@@ -65,7 +65,7 @@ def test_packed_descriptor_matches_c_layout(tmp_path, quant, name):
 
 def linear_desc(quant, **change):
     f = dict(size=quant.LINEAR_DESC.size, abi=1, flags=0, device=0, a_type=3, out_type=0, reserved=0, m=4, n=8, k=16,
-             ld_a=16, ld_w=16, ld_out=8, a=P, a_scale=P, w=P, w_scale=P, bias=0, out=P, scratch=0, scratch_bytes=0,
+             ld_a=16, ld_w=16, ld_out=8, a=P, a_scale=P, w=P, w_scale=P, bias=0, out=P, out_scale=0, scratch=0, scratch_bytes=0,
              status=P, stream=0)
     f.update(change)
     return quant.LINEAR_DESC.pack(*f.values())
@@ -73,7 +73,8 @@ def linear_desc(quant, **change):
 
 @pytest.mark.parametrize("change,want", [
     (dict(size=8), INVALID), (dict(abi=2), INVALID), (dict(flags=2), INVALID), (dict(reserved=1), INVALID),
-    (dict(a_type=4), INVALID), (dict(out_type=3), INVALID), (dict(m=-1), INVALID), (dict(n=0), INVALID),
+    (dict(a_type=4), INVALID), (dict(out_type=3), INVALID), (dict(out_type=4), INVALID),
+    (dict(out_scale=P), INVALID), (dict(out_type=3, out_scale=P + 2), INVALID), (dict(m=-1), INVALID), (dict(n=0), INVALID),
     (dict(k=0), INVALID), (dict(ld_a=15), INVALID), (dict(ld_w=15), INVALID), (dict(ld_out=7), INVALID),
     (dict(a=0), INVALID), (dict(w=0), INVALID), (dict(out=0), INVALID), (dict(w_scale=0), INVALID),
     (dict(a_scale=0), INVALID), (dict(a_type=0), INVALID), (dict(status=0), INVALID), (dict(status=P + 2), INVALID),
