@@ -187,6 +187,47 @@ class GroupedGemmTask(_Struct):
                 ("c", C.c_void_p), ("workspace", C.c_void_p)]
 
 
+class QuantizeDesc(_Struct):  # rns8_cuda_quantize_desc, rns8_quant.h
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("flags", C.c_uint32),
+                ("device_id", C.c_int32), ("x_type", C.c_uint32), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("ld_x", C.c_int64), ("ld_q", C.c_int64), ("x", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class LinearDesc(_Struct):  # rns8_cuda_linear_desc, rns8_quant.h
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("flags", C.c_uint32),
+                ("device_id", C.c_int32), ("a_type", C.c_uint32), ("out_type", C.c_uint32), ("reserved", C.c_uint32),
+                ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("ld_a", C.c_int64), ("ld_w", C.c_int64),
+                ("ld_out", C.c_int64), ("a", C.c_void_p), ("a_scale", C.c_void_p), ("w", C.c_void_p),
+                ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p), ("out_scale", C.c_void_p),
+                ("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64), ("status", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class ResidualNormDesc(_Struct):  # rns8_cuda_residual_norm_desc, rns8_quant.h
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("flags", C.c_uint32),
+                ("device_id", C.c_int32), ("type", C.c_uint32), ("weight_type", C.c_uint32), ("scale", C.c_float),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("tokens", C.c_int64), ("dim", C.c_int64),
+                ("groups", C.c_int64), ("ld_x", C.c_int64), ("ld_y", C.c_int64), ("ld_gate", C.c_int64),
+                ("ld_x_out", C.c_int64), ("ld_h", C.c_int64), ("ld_q", C.c_int64), ("x", C.c_void_p),
+                ("y", C.c_void_p), ("post_weight", C.c_void_p), ("pre_weight", C.c_void_p), ("gate", C.c_void_p),
+                ("x_out", C.c_void_p), ("h", C.c_void_p), ("q", C.c_void_p), ("q_scale", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+class ResidualNormBackwardDesc(_Struct):  # rns8_cuda_residual_norm_backward_desc, rns8_quant.h
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("flags", C.c_uint32),
+                ("device_id", C.c_int32), ("type", C.c_uint32), ("weight_type", C.c_uint32), ("scale", C.c_float),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("tokens", C.c_int64), ("dim", C.c_int64),
+                ("groups", C.c_int64), ("ld_d_x_out", C.c_int64), ("ld_d_h", C.c_int64), ("ld_x_out", C.c_int64),
+                ("ld_y", C.c_int64), ("ld_gate", C.c_int64), ("ld_d_x", C.c_int64), ("ld_d_y", C.c_int64),
+                ("ld_d_gate", C.c_int64), ("d_x_out", C.c_void_p), ("d_h", C.c_void_p), ("x_out", C.c_void_p),
+                ("y", C.c_void_p), ("post_weight", C.c_void_p), ("pre_weight", C.c_void_p), ("gate", C.c_void_p),
+                ("d_x", C.c_void_p), ("d_y", C.c_void_p), ("d_post", C.c_void_p), ("d_pre", C.c_void_p),
+                ("d_gate", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64),
+                ("stream", C.c_void_p)]
+
+
 vp = C.c_void_p
 i64 = C.c_int64
 u64 = C.c_uint64
@@ -270,7 +311,7 @@ SIGNATURES = {
     "rns8_cuda_ipc_open": (c_status, [C.c_int, vp, P(vp)]),
     "rns8_cuda_ipc_close": (c_status, [C.c_int, vp]),
     "rns8_cuda_wait_probe": (c_status, [C.c_int, u32, u64, vp, vp]),
-    # 8-bit operators (include/rns8/rns8_quant.h); each takes one packed descriptor
+    # 8-bit operators (include/rns8/rns8_quant.h); each takes one descriptor
     "rns8_cuda_quantize_rows_device": (c_status, [vp]),
     "rns8_cuda_linear_scratch_bytes": (u64, [vp]),
     "rns8_cuda_linear_device": (c_status, [vp]),

@@ -5,6 +5,10 @@ sm_100a only (-gencode arch=compute_100a,code=sm_100a) and linked into
 rns8_b200/_build/librns8.so, which is what the Python bindings, the tests and
 bench.py load. Object files are rebuilt when a source or header is newer.
 
+Where torch is installed, the torch binding of the 8-bit operators
+(csrc/torch/quant_torch.cpp) is compiled against it by the host compiler into
+rns8_b200/_build/_quant_torch.so; the library itself knows no torch.
+
     python -m rns8_b200.build [--force] [--ptxas-verbose]
 """
 
@@ -12,10 +16,12 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -23,6 +29,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = BUILD / "librns8.so"
+TORCH_SRC = CSRC / "torch" / "quant_torch.cpp"
+TORCH_LIB = BUILD / "_quant_torch.so"
 INCLUDE = ROOT / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -92,7 +100,37 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int | None = N
             raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     if ptxas_verbose:
         print("\n".join(logs))
+    build_torch_binding(force)
     return LIB
+
+
+def build_torch_binding(force: bool = False) -> Path | None:
+    """Compile the torch binding; None where torch is not installed. It is built
+    again when its sources, torch or the Python it was built for change."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    stamp = BUILD / "_quant_torch.stamp"
+    built_for = f"{torch.__version__} {sys.version}"
+    newest = max(p.stat().st_mtime for p in (TORCH_SRC, INCLUDE / "rns8" / "rns8_quant.h"))
+    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == built_for
+            and TORCH_LIB.stat().st_mtime >= newest):
+        return TORCH_LIB
+    compiler = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else "g++"
+    cuda = Path(nvcc()).resolve().parents[1]
+    include = [INCLUDE, root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               sysconfig.get_paths()["include"], cuda / "include"]
+    cmd = [compiler, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in include),
+           str(TORCH_SRC), "-o", str(TORCH_LIB), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python",
+           "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"torch binding failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    stamp.write_text(built_for)
+    return TORCH_LIB
 
 
 def main() -> int:

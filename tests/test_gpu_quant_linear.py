@@ -260,7 +260,7 @@ def test_leading_dimensions_and_empty_batches(quant):
 def test_output_leading_dimension_and_offsets_past_32_bits(quant):
     """Rows of the output (and of the activations) 3e9 bytes apart, through the
     C entry; what lies between rows is untouched."""
-    from rns8_b200.abi import lib
+    from rns8_b200 import abi
 
     m, n, k, ld = 3, 40, 64, 1_500_000_000
     a, s, w, ws, b = operands(m, n, k, 21)
@@ -268,13 +268,14 @@ def test_output_leading_dimension_and_offsets_past_32_bits(quant):
     view_a = torch.as_strided(far_a, (m, k), (ld, 1))
     view_a.copy_(a)
     out = torch.zeros(2 * ld + n + 8, dtype=torch.bfloat16, device="cuda")
-    args = [quant.LINEAR_DESC.size, 1, 0, 0, 3, 0, 0, m, n, k, ld, k, ld, view_a.data_ptr(), s.data_ptr(), w.data_ptr(),
-            ws.data_ptr(), b.data_ptr(), out.data_ptr(), 0, 0, 0, quant.device_status(0).data_ptr(),
-            torch.cuda.current_stream().cuda_stream]
-    need = lib().rns8_cuda_linear_scratch_bytes(quant.LINEAR_DESC.pack(*args))
+    d = abi.LinearDesc()
+    d.a_type, d.m, d.n, d.k, d.ld_a, d.ld_w, d.ld_out = 3, m, n, k, ld, k, ld
+    d.a, d.a_scale, d.w, d.w_scale, d.bias, d.out = (t.data_ptr() for t in (view_a, s, w, ws, b, out))
+    d.status, d.stream = quant.device_status(0).data_ptr(), torch.cuda.current_stream().cuda_stream
+    need = abi.lib().rns8_cuda_linear_scratch_bytes(C.byref(d))
     scratch = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
-    args[20:22] = scratch.data_ptr(), need
-    assert lib().rns8_cuda_linear_device(quant.LINEAR_DESC.pack(*args)) == 0
+    d.scratch, d.scratch_bytes = scratch.data_ptr(), need
+    assert abi.lib().rns8_cuda_linear_device(C.byref(d)) == 0
     got = torch.as_strided(out, (m, n), (ld, 1))
     check_close(got, *linear_ref(a, s, w, ws, b, False), torch.bfloat16)
     assert int(torch.count_nonzero(out[n:n + 4096])) == 0 and int(torch.count_nonzero(out[ld - 4096:ld])) == 0
@@ -283,19 +284,22 @@ def test_output_leading_dimension_and_offsets_past_32_bits(quant):
 
 @pytest.mark.parametrize("m", [5, 150])
 def test_scratch_too_small_is_refused(quant, m):
-    from rns8_b200.abi import lib
+    from rns8_b200 import abi
 
     x = torch.ones(m, 35, dtype=torch.bfloat16, device="cuda")
     _, _, w, ws, _ = operands(1, 33, 35, 2)
     out = torch.zeros(m, 33, dtype=torch.bfloat16, device="cuda")
-    args = [quant.LINEAR_DESC.size, 1, 0, 0, 0, 0, 0, m, 33, 35, 35, 35, 33, x.data_ptr(), 0, w.data_ptr(), ws.data_ptr(),
-            0, out.data_ptr(), 0, 0, 0, quant.device_status(0).data_ptr(), 0]
-    need = lib().rns8_cuda_linear_scratch_bytes(quant.LINEAR_DESC.pack(*args))
-    if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
-        args[20:22] = scratch.data_ptr(), need - 1
-        assert lib().rns8_cuda_linear_device(quant.LINEAR_DESC.pack(*args)) == 7
-        assert int(torch.count_nonzero(out)) == 0
+    d = abi.LinearDesc()
+    d.m, d.n, d.k, d.ld_a, d.ld_w, d.ld_out = m, 33, 35, 35, 35, 33
+    d.a, d.w, d.w_scale, d.out = (t.data_ptr() for t in (x, w, ws, out))
+    d.status, d.stream = quant.device_status(0).data_ptr(), torch.cuda.current_stream().cuda_stream
+    need = abi.lib().rns8_cuda_linear_scratch_bytes(C.byref(d))
+    assert need > 0
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    d.scratch, d.scratch_bytes = scratch.data_ptr(), need - 1
+    assert abi.lib().rns8_cuda_linear_device(C.byref(d)) == 7
+    torch.cuda.synchronize()
+    assert int(torch.count_nonzero(out)) == 0
 
 
 @pytest.mark.parametrize("m", [1, 50, 600])
