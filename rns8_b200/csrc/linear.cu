@@ -13,43 +13,16 @@ namespace {
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0; }
 
-// dst rows (ld a multiple of 16) from src rows of any alignment, 16 bytes a
-// thread: the five aligned words around them, shifted into place (1001 x 2040:
-// 3.7 us byte by byte). Bytes past cols are zero; where a word would reach
-// outside the matrix the bytes are read one by one.
-__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ src, int64_t rows, int64_t cols,
-                                                         int64_t ld, int8_t* __restrict__ dst, int64_t ld_dst) {
+__global__ void __launch_bounds__(256) align_rows_kernel(const AlignRows job) {
   wait_previous_launch();
   allow_next_launch();
-  const int64_t per_row = ld_dst / 16, total = rows * per_row;
-  const int8_t* end = src + (rows - 1) * ld + cols;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * 16;
-    const int8_t* from = src + r * ld + c;
-    const uint32_t shift = reinterpret_cast<uintptr_t>(from) % 4 * 8;
-    const int8_t* base = from - shift / 8;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (c + 16 <= cols && base >= src && base + 20 <= end) {
-      uint32_t v[5];
-#pragma unroll
-      for (int k = 0; k < 5; ++k) v[k] = reinterpret_cast<const uint32_t*>(base)[k];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], shift);
-    } else {
-#pragma unroll
-      for (int b = 0; b < 16; ++b)
-        if (c + b < cols) w[b / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[b])) << (8 * (b % 4));
-    }
-    *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  align_rows(job, static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x,
+             static_cast<int64_t>(gridDim.x) * blockDim.x);
 }
-
-cudaError_t align_rows(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ld_dst,
-                       int sm_count, cudaStream_t stream) {
-  const int64_t chunks = rows * (ld_dst / 16);
+cudaError_t launch_align(const AlignRows& job, int sm_count, cudaStream_t stream) {
+  const int64_t chunks = job.rows * (job.ld_dst / 16);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>((chunks + 255) / 256, sm_count * 16));
-  return launch_chained(align_rows_kernel, dim3(grid), 256, 0, 1, stream, src, rows, cols, ld, dst, ld_dst);
+  return launch_chained(align_rows_kernel, dim3(grid), 256, 0, 1, stream, job);
 }
 
 // What a call needs around its product, and where in scratch.
@@ -84,28 +57,29 @@ uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d) { return plan(d).b
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream) {
   const Steps s = plan(d);
   LinearArgs p{static_cast<const int8_t*>(d.a), d.w, d.a_scale, d.w_scale, d.bias, d.out, d.m, d.n, d.k, d.ld_a, d.ld_w,
-               d.ld_out, d.out_type, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, s.quantize, d.status};
+               d.ld_out, d.out_type, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, false, d.status};
   int8_t* scratch = reinterpret_cast<int8_t*>(round_up(reinterpret_cast<uintptr_t>(d.scratch), 256));
   cudaError_t e = cudaSuccess;
+  const AlignRows weights{d.w, scratch, s.w_rows, d.k, d.ld_w, s.ld};
   if (s.align_w) {
-    e = align_rows(d.w, s.w_rows, d.k, d.ld_w, scratch, s.ld, sm_count, stream);
-    if (e != cudaSuccess) return e;
     p.w = scratch;
     p.ld_w = s.ld;
+    if (!s.quantize) e = launch_align(weights, sm_count, stream);
   }
-  if (s.align_a || s.quantize) {
+  if (e == cudaSuccess && (s.align_a || s.quantize)) {
     int8_t* q = scratch + s.at_a;
     float* scale = reinterpret_cast<float*>(scratch + s.at_scale);
     if (s.quantize) {
-      e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, q, s.ld, scale, stream);
+      e = quantize_rows(d.a, d.a_type, d.m, d.k, d.ld_a, q, s.ld, scale, stream, s.align_w ? &weights : nullptr);
       p.a_scale = scale;
+      p.after_quantize = !s.align_w;
     } else {
-      e = align_rows(p.a, d.m, d.k, d.ld_a, q, s.ld, sm_count, stream);
+      e = launch_align(AlignRows{p.a, q, d.m, d.k, d.ld_a, s.ld}, sm_count, stream);
     }
-    if (e != cudaSuccess) return e;
     p.a = q;
     p.ld_a = s.ld;
   }
+  if (e != cudaSuccess) return e;
   if (!s.quantize_out) return linear_tc(p, sm_count, stream);
   p.out = scratch + s.at_out;
   p.out_type = RNS8_CUDA_TYPE_F32;

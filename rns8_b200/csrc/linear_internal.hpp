@@ -17,7 +17,7 @@ struct LinearArgs {
   int64_t m, n, k, ld_a, ld_w, ld_out;
   uint32_t out_type;
   bool gated;
-  bool after_quantize;  // the previous launch on the stream wrote a and a_scale
+  bool after_quantize;  // the previous launch on the stream wrote a and a_scale, and nothing else that is read here
   uint32_t* status;
 };
 

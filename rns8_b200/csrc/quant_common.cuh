@@ -183,6 +183,40 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int cols, int v, int
   }
 }
 
+// ---- rows on 16-byte boundaries -------------------------------------------------------
+// dst rows (ld_dst a multiple of 16) from int8 src rows of any alignment, 16
+// bytes a thread: the five aligned words around them, shifted into place (1001
+// x 2040 byte by byte: 3.7 us, this 2.0). Bytes past cols are zero; where a word
+// would reach outside the matrix the bytes are read one by one.
+struct AlignRows {
+  const int8_t* src;
+  int8_t* dst;
+  int64_t rows, cols, ld, ld_dst;
+};
+__device__ __forceinline__ void align_rows(const AlignRows& j, int64_t first, int64_t step) {
+  const int64_t per_row = j.ld_dst / 16, total = j.rows * per_row;
+  const int8_t* end = j.src + (j.rows - 1) * j.ld + j.cols;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+    const int8_t* from = j.src + r * j.ld + c;
+    const uint32_t shift = reinterpret_cast<uintptr_t>(from) % 4 * 8;
+    const int8_t* base = from - shift / 8;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (c + 16 <= j.cols && base >= j.src && base + 20 <= end) {
+      uint32_t v[5];
+#pragma unroll
+      for (int k = 0; k < 5; ++k) v[k] = reinterpret_cast<const uint32_t*>(base)[k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], shift);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 16; ++b)
+        if (c + b < j.cols) w[b / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[b])) << (8 * (b % 4));
+    }
+    *reinterpret_cast<uint4*>(j.dst + r * j.ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // ---- quantisation rule ------------------------------------------------------------
 // Magnitudes are compared by their bits: for non-negative floats the unsigned
 // order of the bits is the numeric order, and a NaN is above everything, so a

@@ -10,8 +10,11 @@
 
 namespace rns8cuda {
 
+// With `align` the same launch also copies another int8 matrix's rows to
+// 16-byte boundaries (quant_common.cuh).
+struct AlignRows;
 cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q,
-                          int64_t ld_q, float* scale, cudaStream_t stream);
+                          int64_t ld_q, float* scale, cudaStream_t stream, const AlignRows* align = nullptr);
 
 uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d);
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream);

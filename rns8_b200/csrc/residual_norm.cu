@@ -412,11 +412,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         gate_gradient<ALIGNED, W>(p, gate, j, n, tid, acc[j], acc_post[j]);
         float* out = p.part_gate ? p.part_gate + item * p.dim
                                  : (p.dgate ? static_cast<float*>(p.dgate) + group * p.ld_dgate : nullptr);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = row_index<ALIGNED>(j, e, n, tid);
-          if (out && i < p.dim) out[i] = e % 2 ? acc[j][e / 2].v.y : acc[j][e / 2].v.x;
-        }
+        if (out) store8<ALIGNED>(out, p.dim, j, n, tid, acc[j]);
       }
     }
   }
@@ -608,16 +604,13 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
                             : (p.dgate ? static_cast<float*>(p.dgate) + item / chunks * p.ld_dgate : nullptr);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int i = (j * n + tid) * 8;
       F2 post[4] = {};
       if (dp && item != static_cast<int>(blockIdx.x)) load8<true>(dp, p.dim, j, n, tid, post);
       gate_gradient<true, W>(p, gate, j, n, tid, acc[j], post);
       if (dp) store8<true>(dp, p.dim, j, n, tid, post);
+      if (dg) store8<true>(dg, p.dim, j, n, tid, acc[j]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (dg && i < p.dim) dg[i + 2 * e] = acc[j][e].v.x, dg[i + 2 * e + 1] = acc[j][e].v.y;
-        acc[j][e] = f2(0.0f);
-      }
+      for (int e = 0; e < 4; ++e) acc[j][e] = f2(0.0f);
     }
   }
 #pragma unroll
@@ -630,39 +623,51 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
 }
 
 // out[g][c] = sum over the group's `count` consecutive rows of part. A block
-// sums 32 columns with 16 row lanes, always in the same order. blockIdx.z picks
-// one of three sums.
+// sums 32 columns, four a thread, over 32 row lanes, always in the same order;
+// four rows a lane are on their way at once. blockIdx.z picks one of three sums.
 struct Sums {
   const float* part[3];
   float* out[3];
   int64_t count[3], groups[3], ld_out[3];
   int dim;
 };
-constexpr int kSumLanes = 16;
-__global__ void __launch_bounds__(32 * kSumLanes) sum_rows_kernel(const Sums p) {
-  __shared__ float s[kSumLanes][33];
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const Sums p) {
+  __shared__ float4 s[kSumThreads / 32][8];
   const int z = blockIdx.z;
   wait_previous_launch();
   allow_next_launch();
   if (!p.out[z]) return;
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
+  const int c = blockIdx.x * 32 + threadIdx.x % 8 * 4, lane = threadIdx.x / 8;
+  const bool whole = p.dim % 4 == 0;
   for (int64_t g = blockIdx.y; g < p.groups[z]; g += gridDim.y) {
-    float v[4] = {};
     const float* part = p.part[z] + g * p.count[z] * p.dim + c;
-    if (c < p.dim) {
-      int64_t r = lane;
-      for (; r + 3 * kSumLanes < p.count[z]; r += 4 * kSumLanes)
+    float4 v = make_float4(0, 0, 0, 0);
+    auto add = [&](const float4& a) { v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w; };
+    auto row = [&](int64_t r) {
+      const float* at = part + r * p.dim;
+      if (whole) return *reinterpret_cast<const float4*>(at);
+      return make_float4(at[0], c + 1 < p.dim ? at[1] : 0.0f, c + 2 < p.dim ? at[2] : 0.0f, c + 3 < p.dim ? at[3] : 0.0f);
+    };
+    if (c < p.dim)
+      for (int64_t r = lane; r < p.count[z]; r += 4 * 32) {
+        float4 a[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += part[(r + i * kSumLanes) * p.dim];
-      for (; r < p.count[z]; r += kSumLanes) v[0] += part[r * p.dim];
-    }
-    s[lane][threadIdx.x % 32] = (v[0] + v[1]) + (v[2] + v[3]);
+        for (int i = 0; i < 4; ++i) a[i] = r + i * 32 < p.count[z] ? row(r + i * 32) : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(a[i]);
+      }
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1)
+      add(make_float4(__shfl_xor_sync(0xFFFFFFFFu, v.x, o), __shfl_xor_sync(0xFFFFFFFFu, v.y, o),
+                      __shfl_xor_sync(0xFFFFFFFFu, v.z, o), __shfl_xor_sync(0xFFFFFFFFu, v.w, o)));
+    if (threadIdx.x % 32 < 8) s[threadIdx.x / 32][threadIdx.x % 8] = v;
     __syncthreads();
-    if (lane == 0 && c < p.dim) {
+    if (threadIdx.x < 32 && blockIdx.x * 32 + threadIdx.x < p.dim) {
       float all = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kSumLanes; ++i) all += s[i][threadIdx.x];
-      p.out[z][g * p.ld_out[z] + c] = all;
+      for (int w = 0; w < kSumThreads / 32; ++w) all += reinterpret_cast<const float*>(s[w])[threadIdx.x];
+      p.out[z][g * p.ld_out[z] + blockIdx.x * 32 + threadIdx.x] = all;
     }
     __syncthreads();
   }
@@ -757,7 +762,9 @@ Split split_tokens(const rns8_cuda_residual_norm_backward_desc& d, int sm_count)
   s.per_token = d.gate && d.groups == d.tokens;
   s.groups = (s.per_token || !d.gate) ? 1 : d.groups;
   s.rows_per_group = d.tokens / s.groups;
-  s.chunks = std::min(s.rows_per_group, (target + s.groups - 1) / s.groups);
+  // No more items than blocks where the groups allow it: a second item would
+  // double a block's time.
+  s.chunks = std::min(s.rows_per_group, std::max<int64_t>(1, target / s.groups));
   s.rows_per_item = (s.rows_per_group + s.chunks - 1) / s.chunks;
   s.chunks = (s.rows_per_group + s.rows_per_item - 1) / s.rows_per_item;
   s.items = s.groups * s.chunks;
@@ -861,9 +868,11 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.post_weight, 0, w) && aligned_rows(d.pre_weight, 0, w) &&
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
                        aligned_rows(d.d_y, d.ld_d_y, e) &&
-                       (!s.per_token || aligned_rows(d.d_gate, d.ld_d_gate, e));
+                       aligned_rows(d.d_gate, d.ld_d_gate, s.per_token ? e : sizeof(float));
   const Stream st = backward_stream(p.dim, e);
-  const bool streamed = aligned && p.dim <= 8192 && st.stages > 0;
+  // A block with one narrow row gains nothing from the ring and waits for its
+  // copies (us: 16 x 2048 direct 6.9, streamed 8.3; 16 x 8192 19.3 and 15.4).
+  const bool streamed = aligned && p.dim <= 8192 && st.stages > 0 && !(d.tokens < sm_count && p.dim <= 2048);
   const int vectors = (p.dim + 7) / 8 <= kMaxThreads ? 1 : 4;
   auto launch_stream = [&](auto t, auto wt, auto nv, auto per_token) {
     auto kernel =
@@ -886,7 +895,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   if (err != cudaSuccess) return err;
   if (sums.out[0] || sums.out[1] || sums.out[2]) {
     const unsigned gy = static_cast<unsigned>(std::min<int64_t>(sums.out[2] ? s.groups : 1, 1024));
-    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), 32 * kSumLanes, 0, 1, stream, sums);
+    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), kSumThreads, 0, 1, stream, sums);
   }
   return err;
 }

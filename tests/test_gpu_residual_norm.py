@@ -200,7 +200,8 @@ def check_backward(quant, t, dxo, dh, dtype, scale=0.7, eps=1e-5, offset=0.0):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("tokens,dim,groups", SHAPES + [(1000, 64, 500), (777, 136, 1), (2000, 2048, 2)])
+@pytest.mark.parametrize("tokens,dim,groups", SHAPES + [(1000, 64, 500), (777, 136, 1), (2000, 2048, 2),
+                                                           (3000, 64, 1500), (900, 4096, 300), (450, 130, 150)])
 def test_backward(quant, tokens, dim, groups, dtype):
     t = make(tokens, dim, groups, dtype)
     g = rng(dim)
