@@ -13,7 +13,31 @@
 namespace rns8cuda {
 namespace {
 
-template <typename T, bool ALIGNED, int NV>
+// How a row is read: as 16-byte words; as words of a 16-bit row that starts
+// anywhere, the five around each vector shifted into place; element by element.
+enum class Read { Aligned, Shifted, Elements };
+
+// Vector of a 16-bit row at i, which may be the row's last and short; `first`
+// and `end` bound the matrix.
+template <typename T>
+__device__ __forceinline__ void load_shifted(const T* row, int i, int cols, const T* first, const T* end, F2 (&v)[4]) {
+  const T* from = row + i;
+  const bool odd = reinterpret_cast<uintptr_t>(from) % 4 != 0;
+  const T* base = from - (odd ? 1 : 0);
+  if (i + 8 <= cols && base >= first && base + 10 <= end) {
+    uint32_t w[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = reinterpret_cast<const uint32_t*>(base)[k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = unpack2<T>(__funnelshift_r(w[k], w[k + 1], odd ? 16 : 0));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = f2(i + 2 * k < cols ? to_f32(from[2 * k]) : 0.0f, i + 2 * k + 1 < cols ? to_f32(from[2 * k + 1]) : 0.0f);
+  }
+}
+
+template <typename T, Read READ, int NV>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, int cols, int64_t ld_x,
                                                              int8_t* __restrict__ q, int64_t ld_q,
                                                              float* __restrict__ scale, int64_t rows,
@@ -30,13 +54,28 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict
   F2 v[NV][4];
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) load8<ALIGNED>(xr, cols, j, blockDim.x, threadIdx.x, v[j]);
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (READ == Read::Shifted)
+      load_shifted<T>(xr, (j * blockDim.x + threadIdx.x) * 8, cols, x, x + (rows - 1) * ld_x + cols, v[j]);
+    else
+      load8<READ == Read::Aligned>(xr, cols, j, blockDim.x, threadIdx.x, v[j]);
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) top = max(top, magnitude_bits(v[j]));
   const RowScale rs = make_row_scale(block_max(top, slots));
   if (threadIdx.x == 0) scale[row] = rs.scale;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) store_q8<ALIGNED>(q + row * ld_q, cols, j, blockDim.x, threadIdx.x, v[j], rs.inv);
+  for (int j = 0; j < NV; ++j) {
+    const int i = (j * blockDim.x + threadIdx.x) * 8;
+    if (READ != Read::Shifted || i + 8 <= cols) {
+      store_q8<READ != Read::Elements>(q + row * ld_q, cols, j, blockDim.x, threadIdx.x, v[j], rs.inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < cols)
+          q[row * ld_q + i + e] = static_cast<int8_t>(quantize_one(e % 2 ? v[j][e / 2].v.y : v[j][e / 2].v.x, rs.inv));
+    }
+  }
 }
 
 template <typename T>
@@ -64,8 +103,8 @@ __global__ void __launch_bounds__(1024) quantize_long_rows_kernel(const T* __res
 template <typename T>
 cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale,
                    const AlignRows* align, cudaStream_t stream) {
-  const bool aligned = cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(q) % 8 == 0 && ld_q % 8 == 0;
+  const bool q_words = reinterpret_cast<uintptr_t>(q) % 8 == 0 && ld_q % 8 == 0;
+  const bool aligned = q_words && cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_x * sizeof(T) % 16 == 0;
   // Blocks for the other matrix: 16 bytes a thread, four rounds of the GPU at most.
   auto grid = [&](unsigned threads) {
     int64_t blocks = 0;
@@ -77,19 +116,24 @@ cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ld_x, int8_t*
     return launch_chained(quantize_long_rows_kernel<T>, grid(1024), 1024, 0, 1, stream, x, cols, ld_x, q, ld_q, scale,
                           rows, job);
   const int c = static_cast<int>(cols), vecs = (c + 7) / 8;
-  auto go = [&](auto nv, auto al) {
+  auto go = [&](auto nv, auto read) {
     constexpr int NV = decltype(nv)::value;
     const unsigned threads = static_cast<unsigned>(std::max(32, ((vecs + NV - 1) / NV + 31) / 32 * 32));
-    return launch_chained(quantize_rows_kernel<T, decltype(al)::value, NV>, grid(threads), threads, 0, 1, stream, x, c,
+    return launch_chained(quantize_rows_kernel<T, decltype(read)::value, NV>, grid(threads), threads, 0, 1, stream, x, c,
                           ld_x, q, ld_q, scale, rows, job);
   };
-  auto pick = [&](auto al) {
+  auto pick = [&](auto read) {
     const int nv = row_vectors(rows, vecs);
-    if (nv == 1) return go(std::integral_constant<int, 1>{}, al);
-    if (nv == 2) return go(std::integral_constant<int, 2>{}, al);
-    return go(std::integral_constant<int, 4>{}, al);
+    if (nv == 1) return go(std::integral_constant<int, 1>{}, read);
+    if (nv == 2) return go(std::integral_constant<int, 2>{}, read);
+    return go(std::integral_constant<int, 4>{}, read);
   };
-  return aligned ? pick(std::true_type{}) : pick(std::false_type{});
+  if (aligned) return pick(std::integral_constant<Read, Read::Aligned>{});
+  if constexpr (sizeof(T) == 2) {
+    // 1500 x 5713 bf16: 28 us element by element.
+    if (q_words) return pick(std::integral_constant<Read, Read::Shifted>{});
+  }
+  return pick(std::integral_constant<Read, Read::Elements>{});
 }
 
 }  // namespace
