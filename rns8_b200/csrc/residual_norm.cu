@@ -809,7 +809,8 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, c
                        : launch_stream(t, wt, std::integral_constant<int, 2>{});
     });
   }
-  const int vectors = row_vectors(d.tokens, (p.dim + 7) / 8);
+  // Element by element a thread has eight times the accesses: more threads.
+  const int vecs = (p.dim + 7) / 8, vectors = aligned ? row_vectors(d.tokens, vecs) : (vecs <= kMaxThreads ? 1 : 4);
   return dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
     return launch_chained(residual_norm_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
