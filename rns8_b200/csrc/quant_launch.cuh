@@ -6,7 +6,8 @@
 // kernel may write or read) and then lets the next one come up the same way.
 // A chain of short kernels so loses most of its launch gaps. Because a kernel
 // signals only after its own wait, whatever ran two launches back is complete
-// when a kernel starts.
+// when its successor starts. (A product after its own quantisation signals at
+// once and waits later; what follows it waits for it as for any other.)
 #pragma once
 
 #include <cuda_runtime.h>

@@ -153,6 +153,7 @@ class _ResidualNorm(torch.autograd.Function):
         return x_out, h
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_x_out, d_h):
         x_out, y, post_weight, pre_weight, gate = ctx.saved_tensors
         if d_x_out is None and d_h is None:
