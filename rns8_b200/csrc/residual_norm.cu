@@ -5,12 +5,12 @@
 // on it, so HBM is to bound them; what stands in the way is that a row must be
 // reduced before any of it can be written. Two forms each:
 //
-//   streamed  For rows on 16-byte boundaries and many tokens: persistent
-//             blocks whose rows arrive in shared memory through a ring of bulk
-//             copies, so that the next tokens' bytes are on their way while
-//             this token is reduced.
-//   direct    For the rest (unaligned rows, few tokens, very wide rows): a row
-//             read straight into registers.
+//   streamed  For many tokens: persistent blocks whose rows arrive in shared
+//             memory through a ring of bulk copies, so that the next tokens'
+//             bytes are on their way while this token is reduced.
+//   direct    For few tokens, for very wide rows, and forward for rows that do
+//             not start on 16-byte boundaries: a row read straight into
+//             registers.
 #include <algorithm>
 #include <atomic>
 
@@ -33,7 +33,82 @@ struct Forward {
   float* q_scale;
   float scale, eps, offset, inv_dim;
   int dim;
+  bool q_words;
 };
+
+// How a kernel reads and writes rows.
+//   Words     On 16-byte boundaries, the width a multiple of 8.
+//   Shifted   The rest (odd widths, slices): vectors shifted into place (4000 x
+//             8191 bf16 98 us, element by element 203; 1 x 1001 2.7 and 4.0).
+//   Elements  The rest where a vector a thread holds a row of floats (2000 x
+//             1001 9.2 us, shifted 10.7; wider ones 249 and 171 at 8000 x 5001)
+//             and in the streamed backward form: shared memory reads any
+//             alignment alike, and shifting four rows costs more issue (4000 x
+//             8191 f32 198 us, shifted 250).
+enum class Access { Words, Shifted, Elements };
+
+// Index of element e of this thread's vector j.
+template <Access A>
+__device__ __forceinline__ int element_index(int j, int e, int n, int tid) {
+  return row_index<A != Access::Elements>(j, e, n, tid);
+}
+// Vector j of this thread's part of a row; elements at or past dim are zero.
+template <Access A, typename T>
+__device__ __forceinline__ Raw8<T> load_raw(const T* row, int dim, int j, int n, int tid) {
+  if constexpr (A == Access::Words) {
+    const int i = (j * n + tid) * 8;
+    Raw8<T> v;
+    v.load(row + i, i < dim);
+    return v;
+  } else if constexpr (A == Access::Shifted) {
+    return load_shifted<T>(row, dim, (j * n + tid) * 8);
+  } else {
+    F2 v[4];
+    load8<false>(row, dim, j, n, tid, v);
+    Raw8<T> raw;
+    raw.set(v);
+    return raw;
+  }
+}
+template <Access A, typename T>
+__device__ __forceinline__ void load_row(const T* row, int dim, int j, int n, int tid, F2 (&v)[4]) {
+  if constexpr (A == Access::Elements) {
+    load8<false>(row, dim, j, n, tid, v);
+  } else {
+    const Raw8<T> raw = load_raw<A>(row, dim, j, n, tid);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = raw.pair(e);
+  }
+}
+template <Access A, typename T>
+__device__ __forceinline__ void store_row(T* row, int dim, int j, int n, int tid, const F2 (&v)[4]) {
+  if constexpr (A == Access::Shifted) {
+    Raw8<T> raw;
+    raw.set(v);
+    store_shifted<T>(row, dim, (j * n + tid) * 8, raw);
+  } else {
+    store8<A == Access::Words>(row, dim, j, n, tid, v);
+  }
+}
+// Rows of partial sums, padded to whole vectors.
+template <Access A>
+__device__ __forceinline__ void store_partial(float* row, int dim, int j, int n, int tid, const F2 (&v)[4]) {
+  store8<A != Access::Elements>(row, dim, j, n, tid, v);
+}
+// int8 values of a vector; q_words: q's rows are on 8-byte boundaries.
+template <Access A>
+__device__ __forceinline__ void store_row_q8(int8_t* row, bool q_words, int dim, int j, int n, int tid,
+                                             const F2 (&v)[4], float inv) {
+  if (A == Access::Words || (A == Access::Shifted && q_words && (j * n + tid) * 8 + 8 <= dim)) {
+    store_q8<true>(row, dim, j, n, tid, v, inv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = element_index<A>(j, e, n, tid);
+      if (i < dim) row[i] = static_cast<int8_t>(quantize_one(e % 2 ? v[e / 2].v.y : v[e / 2].v.x, inv));
+    }
+  }
+}
 
 // Sum of a row's squares over the block.
 template <int NV>
@@ -50,7 +125,7 @@ __device__ __forceinline__ float row_squares(const F2 (&v)[NV][4], SumSlots<1>& 
 
 // x += f * y * (offset + post) * gate for one vector; f holds scale and y's row
 // factor. The options' branches are taken per vector.
-template <bool ALIGNED, typename T, typename W>
+template <Access A, typename T, typename W>
 __device__ __forceinline__ void add_update(const Forward& p, const W* gate, float f, int j, int n, int tid,
                                            const F2 (&y)[4], F2 (&x)[4]) {
   F2 m[4];
@@ -58,41 +133,41 @@ __device__ __forceinline__ void add_update(const Forward& p, const W* gate, floa
   for (int e = 0; e < 4; ++e) m[e] = f2(f);
   if (p.post) {
     F2 w[4];
-    load8<ALIGNED>(static_cast<const W*>(p.post), p.dim, j, n, tid, w);
+    load_row<A>(static_cast<const W*>(p.post), p.dim, j, n, tid, w);
 #pragma unroll
     for (int e = 0; e < 4; ++e) m[e] = m[e] * (w[e] + f2(p.offset));
   }
   if (p.gate) {
     F2 g[4];
-    load8<ALIGNED>(gate, p.dim, j, n, tid, g);
+    load_row<A>(gate, p.dim, j, n, tid, g);
 #pragma unroll
     for (int e = 0; e < 4; ++e) m[e] = m[e] * g[e];
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = fma(y[e], m[e], x[e]);
 }
-template <bool ALIGNED, typename W>
+template <Access A, typename W>
 __device__ __forceinline__ void normalize(const Forward& p, float rho, int j, int n, int tid, F2 (&x)[4]) {
   F2 w[4];
-  load8<ALIGNED>(static_cast<const W*>(p.pre), p.dim, j, n, tid, w);
+  load_row<A>(static_cast<const W*>(p.pre), p.dim, j, n, tid, w);
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = x[e] * (f2(rho) * (w[e] + f2(p.offset)));
 }
 // Largest magnitude of a vector. Elements past the row are left out: they are
 // zero, but a row that holds an infinity has rho = 0 or NaN.
-template <bool ALIGNED>
+template <Access A>
 __device__ __forceinline__ uint32_t row_magnitude(const F2 (&v)[4], int dim, int j, int n, int tid) {
-  if (ALIGNED) return (j * n + tid) * 8 < dim ? magnitude_bits(v) : 0u;
+  if (A == Access::Words) return (j * n + tid) * 8 < dim ? magnitude_bits(v) : 0u;
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (row_index<ALIGNED>(j, e, n, tid) < dim) top = max(top, magnitude_bits(e % 2 ? v[e / 2].v.y : v[e / 2].v.x));
+    if (element_index<A>(j, e, n, tid) < dim) top = max(top, magnitude_bits(e % 2 ? v[e / 2].v.y : v[e / 2].v.x));
   return top;
 }
 
 // One block per token; the token's row stays in registers from its load to its
 // stores.
-template <typename T, typename W, bool ALIGNED, int NV>
+template <typename T, typename W, Access A, int NV>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const Forward p) {
   __shared__ SumSlots<1> slots[2];
   __shared__ uint32_t max_slots[32];
@@ -106,61 +181,76 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const Forwar
   F2 y[NV][4], x[NV][4];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    load8<ALIGNED>(static_cast<const T*>(p.y) + t * p.ld_y, p.dim, j, n, tid, y[j]);
-    load8<ALIGNED>(static_cast<const T*>(p.x) + t * p.ld_x, p.dim, j, n, tid, x[j]);
+    load_row<A>(static_cast<const T*>(p.y) + t * p.ld_y, p.dim, j, n, tid, y[j]);
+    load_row<A>(static_cast<const T*>(p.x) + t * p.ld_x, p.dim, j, n, tid, x[j]);
   }
   const W* gate = static_cast<const W*>(p.gate) + (p.gate ? t / p.rows_per_gate * p.ld_gate : 0);
   float f = p.scale;
   if (p.post) f *= rsqrtf(row_squares(y, slots[0]) * p.inv_dim + p.eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    add_update<ALIGNED, T, W>(p, gate, f, j, n, tid, y[j], x[j]);
-    store8<ALIGNED>(static_cast<T*>(p.x_out) + t * p.ld_x_out, p.dim, j, n, tid, x[j]);
+    add_update<A, T, W>(p, gate, f, j, n, tid, y[j], x[j]);
+    store_row<A>(static_cast<T*>(p.x_out) + t * p.ld_x_out, p.dim, j, n, tid, x[j]);
   }
   if (!p.pre) return;
   const float rho = rsqrtf(row_squares(x, slots[1]) * p.inv_dim + p.eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    normalize<ALIGNED, W>(p, rho, j, n, tid, x[j]);
-    if (p.h) store8<ALIGNED>(static_cast<T*>(p.h) + t * p.ld_h, p.dim, j, n, tid, x[j]);
+    normalize<A, W>(p, rho, j, n, tid, x[j]);
+    if (p.h) store_row<A>(static_cast<T*>(p.h) + t * p.ld_h, p.dim, j, n, tid, x[j]);
   }
   if (!p.q) return;
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<ALIGNED>(x[j], p.dim, j, n, tid));
+  for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<A>(x[j], p.dim, j, n, tid));
   const RowScale rs = make_row_scale(block_max(top, max_slots));
   if (tid == 0) p.q_scale[t] = rs.scale;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) store_q8<ALIGNED>(p.q + t * p.ld_q, p.dim, j, n, tid, x[j], rs.inv);
+  for (int j = 0; j < NV; ++j) store_row_q8<A>(p.q + t * p.ld_q, p.q_words, p.dim, j, n, tid, x[j], rs.inv);
 }
 
 // ---- rows through shared memory -----------------------------------------------------
 constexpr int kMaxRing = 8;
 
-// A ring of `stages` slots, each ROWS rows of row_bytes bytes, filled by one
-// thread's bulk copies. A wait that runs out cannot be reported (these calls
+// Room for a row, or for the 16-byte words around one that starts anywhere.
+__host__ __device__ constexpr uint32_t row_room(bool aligned, int dim, uint32_t elem) {
+  return aligned ? dim * elem : (dim * elem + 15) / 16 * 16 + 16;
+}
+__device__ __forceinline__ uint32_t row_offset(const void* row) { return reinterpret_cast<uintptr_t>(row) % 16; }
+// Whether a token's rows are copied: the words around the first and the last
+// may reach outside their matrices (those of the rows between do not, with rows
+// of at least one word). Such tokens are read from global memory.
+template <Access A>
+__device__ __forceinline__ bool copied(int64_t t, int64_t tokens) {
+  return A == Access::Words || (t > 0 && t < tokens - 1);
+}
+
+// A ring of `stages` slots, each room for ROWS rows, filled by one thread's bulk
+// copies of the 16-byte words around them. A wait that runs out cannot be reported (these calls
 // have no status word), so it does not change the result instead: the thread
 // reads its part of that and every later row from global memory.
 template <int ROWS>
 struct RowRing {
   uint8_t* base;
   uint64_t* full;
-  uint32_t row_bytes, stages, stage = 0, phase = 0;
+  uint32_t row_bytes, room, stages, stage = 0, phase = 0;
   uint32_t filled = 0, parity = ~0u;  // slots ever filled, parity of each one's last fill
   bool lost = false;
 
-  __device__ uint8_t* slot(uint32_t s, int row) const { return base + (s * ROWS + row) * row_bytes; }
+  __device__ uint8_t* slot(uint32_t s, int row) const { return base + (s * ROWS + row) * room; }
+  // Bytes of the words around a row.
+  __device__ uint32_t words(const uint8_t* row) const { return (row_offset(row) + row_bytes + 15) & ~15u; }
   // One thread: the rows of one token into slot s (a null row is left out).
   __device__ void fill(uint32_t s, const uint8_t* const (&rows)[ROWS]) {
     uint32_t bytes = 0;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) bytes += rows[r] ? row_bytes : 0;
+    for (int r = 0; r < ROWS; ++r) bytes += rows[r] ? words(rows[r]) : 0;
     mbar_arrive_expect_tx(&full[s], bytes);
     filled |= 1u << s;
     parity ^= 1u << s;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (rows[r]) bulk_load_1d(slot(s, r), rows[r], row_bytes, &full[s]);
+      if (rows[r]) bulk_load_1d(slot(s, r), rows[r] - row_offset(rows[r]), words(rows[r]), &full[s]);
   }
   __device__ void wait() {
     if (!lost) lost = !mbar_wait_bounded(&full[stage], phase);
@@ -184,7 +274,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_stream_kernel(const
   __shared__ uint32_t max_slots[2][32];
   const int n = blockDim.x, tid = threadIdx.x;
   for (int b = 0; b < 4; ++b) clear_slots(slots[b / 2][b % 2]);
-  RowRing<2> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), stages};
+  const uint32_t row_bytes = p.dim * sizeof(T);
+  RowRing<2> ring{ring_bytes, full, row_bytes, row_bytes, stages};
   if (tid == 0) {
     for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
@@ -235,20 +326,20 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_stream_kernel(const
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[j][e] = x[j].pair(e);
-      add_update<true, T, W>(p, gate, f, j, n, tid, y[j], v[j]);
+      add_update<Access::Words, T, W>(p, gate, f, j, n, tid, y[j], v[j]);
       store8<true>(static_cast<T*>(p.x_out) + t * p.ld_x_out, p.dim, j, n, tid, v[j]);
     }
     if (!p.pre) continue;
     const float rho = rsqrtf(row_squares(v, slots[buf][1]) * p.inv_dim + p.eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      normalize<true, W>(p, rho, j, n, tid, v[j]);
+      normalize<Access::Words, W>(p, rho, j, n, tid, v[j]);
       if (p.h) store8<true>(static_cast<T*>(p.h) + t * p.ld_h, p.dim, j, n, tid, v[j]);
     }
     if (!p.q) continue;
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<true>(v[j], p.dim, j, n, tid));
+    for (int j = 0; j < NV; ++j) top = max(top, row_magnitude<Access::Words>(v[j], p.dim, j, n, tid));
     const RowScale rs = make_row_scale(block_max(top, max_slots[buf]));
     if (tid == 0) p.q_scale[t] = rs.scale;
 #pragma unroll
@@ -261,28 +352,28 @@ struct Backward {
   int64_t ld_dxo, ld_dh, ld_x, ld_y, ld_gate, ld_dx, ld_dy, ld_dgate;
   const void *dxo, *dh, *x, *y, *post, *pre, *gate;
   void *dx, *dy, *dgate;
-  float *part_post, *part_pre, *part_gate;  // per-block sums [grid][dim], per-item gate sums [items][dim]
-  int64_t items, chunks, rows_per_item, rows_per_group, rows_per_gate;
+  float *part_post, *part_pre, *part_gate;  // per-block sums [grid][pitch], per-item gate sums [items][pitch]
+  int64_t tokens, items, chunks, rows_per_item, rows_per_group, rows_per_gate;
   float scale, eps, offset, inv_dim;
-  int dim;
+  int dim, pitch;
   bool per_token;  // one gate row per token: d_gate is written token by token
 };
 
 // What the two backward forms share, for one vector of a row.
-template <bool ALIGNED, typename T>
+template <Access A, typename T>
 __device__ __forceinline__ void load_or(const T* row, float none, int dim, int j, int n, int tid, F2 (&v)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = f2(none);
-  if (row) load8<ALIGNED>(row, dim, j, n, tid, v);
+  if (row) load_row<A>(row, dim, j, n, tid, v);
 }
 // a = scale * gate * (offset + post), pre = offset + pre_weight (0 without).
-template <bool ALIGNED, typename W>
+template <Access A, typename W>
 __device__ __forceinline__ void make_factors(const Backward& p, const W* gate, int j, int n, int tid, F2 (&a)[4],
                                              F2 (&pre)[4]) {
   F2 w[4], g[4];
-  load_or<ALIGNED>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
-  load_or<ALIGNED>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
-  load_or<ALIGNED>(static_cast<const W*>(p.pre), -p.offset, p.dim, j, n, tid, pre);
+  load_or<A>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<A>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
+  load_or<A>(static_cast<const W*>(p.pre), -p.offset, p.dim, j, n, tid, pre);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     a[e] = f2(p.scale) * g[e] * (w[e] + f2(p.offset));
@@ -290,12 +381,12 @@ __device__ __forceinline__ void make_factors(const Backward& p, const W* gate, i
   }
 }
 // u dx summed or single -> the gate's gradient in place, post's share added.
-template <bool ALIGNED, typename W>
+template <Access A, typename W>
 __device__ __forceinline__ void gate_gradient(const Backward& p, const W* gate, int j, int n, int tid, F2 (&udx)[4],
                                               F2 (&acc_post)[4]) {
   F2 w[4], g[4];
-  load_or<ALIGNED>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
-  load_or<ALIGNED>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
+  load_or<A>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<A>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     acc_post[e] = fma(f2(p.scale) * g[e], udx[e], acc_post[e]);
@@ -347,11 +438,13 @@ __device__ __forceinline__ void row_gradients(const RowFactors& r, const F2 (&dx
   }
 }
 
+constexpr int kNarrow = 4096;  // widest row of the direct backward form's blocks with a vector a thread
+
 // A block walks items (runs of tokens that share a gate row) and keeps the
 // sums over tokens in registers: for dgate and dpost A = sum of u * dx over an
 // item (both are multiples of it by per-channel factors), for dpre its own.
-template <typename T, typename W, bool ALIGNED, int NV>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const Backward p) {
+template <typename T, typename W, Access A, int NV>
+__global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_norm_backward_kernel(const Backward p) {
   __shared__ SumSlots<6> slots[2];
   const int n = blockDim.x, tid = threadIdx.x;
   clear_slots(slots[0]);
@@ -375,11 +468,11 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         F2 dxo[4], dh[4], x[4], y[4], a[4], pre[4];
       };
       auto load = [&](int j, Vec& v) {
-        load8<ALIGNED>(x, p.dim, j, n, tid, v.x);
-        load8<ALIGNED>(y, p.dim, j, n, tid, v.y);
-        load_or<ALIGNED>(dxo, 0.0f, p.dim, j, n, tid, v.dxo);
-        load_or<ALIGNED>(dh, 0.0f, p.dim, j, n, tid, v.dh);
-        make_factors<ALIGNED, W>(p, gate, j, n, tid, v.a, v.pre);
+        load_row<A>(x, p.dim, j, n, tid, v.x);
+        load_row<A>(y, p.dim, j, n, tid, v.y);
+        load_or<A>(dxo, 0.0f, p.dim, j, n, tid, v.dxo);
+        load_or<A>(dh, 0.0f, p.dim, j, n, tid, v.dh);
+        make_factors<A, W>(p, gate, j, n, tid, v.a, v.pre);
       };
       Vec v;
       RowSums sums{};
@@ -394,11 +487,11 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         if (NV > 1) load(j, v);
         F2 dx[4], dy[4], udx[4];
         row_gradients(r, v.dxo, v.dh, v.x, v.y, v.a, v.pre, dx, dy, udx, acc_pre[j]);
-        store8<ALIGNED>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
-        store8<ALIGNED>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
+        store_row<A>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
+        store_row<A>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
         if (p.per_token) {
-          gate_gradient<ALIGNED, W>(p, gate, j, n, tid, udx, acc_post[j]);
-          if (p.dgate) store8<ALIGNED>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+          gate_gradient<A, W>(p, gate, j, n, tid, udx, acc_post[j]);
+          if (p.dgate) store_row<A>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
@@ -409,17 +502,18 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       const W* gate = static_cast<const W*>(p.gate) + (p.gate ? first / p.rows_per_gate * p.ld_gate : 0);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        gate_gradient<ALIGNED, W>(p, gate, j, n, tid, acc[j], acc_post[j]);
-        float* out = p.part_gate ? p.part_gate + item * p.dim
-                                 : (p.dgate ? static_cast<float*>(p.dgate) + group * p.ld_dgate : nullptr);
-        if (out) store8<ALIGNED>(out, p.dim, j, n, tid, acc[j]);
+        gate_gradient<A, W>(p, gate, j, n, tid, acc[j], acc_post[j]);
+        if (p.part_gate)
+          store_partial<A>(p.part_gate + item * p.pitch, p.dim, j, n, tid, acc[j]);
+        else if (p.dgate)
+          store_row<A>(static_cast<float*>(p.dgate) + group * p.ld_dgate, p.dim, j, n, tid, acc[j]);
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (p.part_post) store8<ALIGNED>(p.part_post + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc_post[j]);
-    if (p.part_pre) store8<ALIGNED>(p.part_pre + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc_pre[j]);
+    if (p.part_post) store_partial<A>(p.part_post + static_cast<int64_t>(blockIdx.x) * p.pitch, p.dim, j, n, tid, acc_post[j]);
+    if (p.part_pre) store_partial<A>(p.part_pre + static_cast<int64_t>(blockIdx.x) * p.pitch, p.dim, j, n, tid, acc_pre[j]);
   }
 }
 
@@ -431,7 +525,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 // a row costs besides its elements (one reduction of six sums) small.
 // With a gate row per token (PER_TOKEN) the gate's words are read beside the
 // token's, and the factors kept are those of the weights alone.
-template <typename T, typename W, int NV, bool PER_TOKEN>
+template <typename T, typename W, Access A, int NV, bool PER_TOKEN>
 __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(const Backward p, uint32_t stages) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];
   __shared__ __align__(8) uint64_t full[kMaxRing];
@@ -439,8 +533,9 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
   const int n = blockDim.x, tid = threadIdx.x;
   clear_slots(slots[0]);
   clear_slots(slots[1]);
-  RowRing<4> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), stages};
-  float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * 4 * ring.row_bytes);  // [NV][4][n]: a, a, pre, pre
+  RowRing<4> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), row_room(A == Access::Words, p.dim, sizeof(T)),
+                   stages};
+  float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * 4 * ring.room);  // [NV][4][n]: a, a, pre, pre
   if (tid == 0) {
     for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
@@ -470,11 +565,13 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
   const T* dh_base = static_cast<const T*>(p.dh);
   const T* x_base = static_cast<const T*>(p.x);
   const T* y_base = static_cast<const T*>(p.y);
+  const T* bases[4] = {dxo_base, dh_base, x_base, y_base};
+  const int64_t lds[4] = {p.ld_dxo, p.ld_dh, p.ld_x, p.ld_y};
   auto fill = [&](uint32_t s, int64_t t) {
-    const uint8_t* rows[4] = {reinterpret_cast<const uint8_t*>(dxo_base ? dxo_base + t * p.ld_dxo : nullptr),
-                              reinterpret_cast<const uint8_t*>(dh_base ? dh_base + t * p.ld_dh : nullptr),
-                              reinterpret_cast<const uint8_t*>(x_base + t * p.ld_x),
-                              reinterpret_cast<const uint8_t*>(y_base + t * p.ld_y)};
+    const bool copy = copied<A>(t, p.tokens);
+    const uint8_t* rows[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) rows[r] = reinterpret_cast<const uint8_t*>(bases[r] && copy ? bases[r] + t * lds[r] : nullptr);
     ring.fill(s, rows);
   };
   Cursor ahead{static_cast<int>(blockIdx.x), 0, 0};
@@ -489,7 +586,7 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       F2 a[4], pre[4];
-      make_factors<true, W>(p, gate, j, n, tid, a, pre);
+      make_factors<A, W>(p, gate, j, n, tid, a, pre);
       float4* f = factors + j * 4 * n + tid;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -519,27 +616,25 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
     Raw8<W> gate_row[PER_TOKEN ? NV : 1];
     if (PER_TOKEN)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int i = (j * n + tid) * 8;
-        gate_row[j].load(static_cast<const W*>(p.gate) + t * p.ld_gate + i, i < p.dim);
-      }
+      for (int j = 0; j < NV; ++j)
+        gate_row[j] = load_raw<A>(static_cast<const W*>(p.gate) + t * p.ld_gate, p.dim, j, n, tid);
     ring.wait();
     Raw8<T> dxo[NV], dh[NV], x[NV], y[NV];
-    auto take = [&](const T* r0, const T* r1, const T* r2, const T* r3) {
+    auto take = [&](auto row) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int i = (j * n + tid) * 8;
-        dxo[j].load(r0 + i, i < p.dim && dxo_base);
-        dh[j].load(r1 + i, i < p.dim && dh_base);
-        x[j].load(r2 + i, i < p.dim);
-        y[j].load(r3 + i, i < p.dim);
+        dxo[j] = dh[j] = Raw8<T>{};
+        if (dxo_base) dxo[j] = load_raw<A>(row(0), p.dim, j, n, tid);
+        if (dh_base) dh[j] = load_raw<A>(row(1), p.dim, j, n, tid);
+        x[j] = load_raw<A>(row(2), p.dim, j, n, tid);
+        y[j] = load_raw<A>(row(3), p.dim, j, n, tid);
       }
     };
-    auto slot = [&](int r) { return reinterpret_cast<const T*>(ring.slot(ring.stage, r)); };
-    if (!ring.lost)  // two branches, so that these are shared-memory loads
-      take(slot(0), slot(1), slot(2), slot(3));
+    // Two branches, so that these are shared-memory loads.
+    if (!ring.lost && copied<A>(t, p.tokens))
+      take([&](int r) { return reinterpret_cast<const T*>(ring.slot(ring.stage, r) + row_offset(bases[r] + t * lds[r])); });
     else
-      take(dxo_base + t * p.ld_dxo, dh_base + t * p.ld_dh, x_base + t * p.ld_x, y_base + t * p.ld_y);
+      take([&](int r) { return bases[r] + t * lds[r]; });
     release_stage_reads();
     RowSums sums{};
 #pragma unroll
@@ -576,8 +671,8 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
           for (int e = 0; e < 4; ++e) a[e] = a[e] * gate_row[j].pair(e);
         row_gradients(r, fdxo, fdh, fx, fy, a, pre, dx, dy, udx, acc_pre[j]);
       }
-      store8<true>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
-      store8<true>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
+      store_row<A>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
+      store_row<A>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
       if (PER_TOKEN) {
         F2 base[4], pre[4];  // scale * (offset + post)
         get_factors(j, base, pre);
@@ -586,7 +681,7 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
           acc[j][e] = fma(f2(p.scale) * gate_row[j].pair(e), udx[e], acc[j][e]);
           udx[e] = base[e] * udx[e];
         }
-        if (p.dgate) store8<true>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+        if (p.dgate) store_row<A>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
@@ -599,16 +694,17 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
     // The item's sums: its gate row's gradient, and its share of post's, which
     // the block adds up over its items in its own row of part_post.
     const W* gate = static_cast<const W*>(p.gate) + (p.gate ? t / p.rows_per_gate * p.ld_gate : 0);
-    float* dp = p.part_post ? p.part_post + static_cast<int64_t>(blockIdx.x) * p.dim : nullptr;
-    float* dg = p.part_gate ? p.part_gate + static_cast<int64_t>(item) * p.dim
-                            : (p.dgate ? static_cast<float*>(p.dgate) + item / chunks * p.ld_dgate : nullptr);
+    float* dp = p.part_post ? p.part_post + static_cast<int64_t>(blockIdx.x) * p.pitch : nullptr;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       F2 post[4] = {};
-      if (dp && item != static_cast<int>(blockIdx.x)) load8<true>(dp, p.dim, j, n, tid, post);
-      gate_gradient<true, W>(p, gate, j, n, tid, acc[j], post);
-      if (dp) store8<true>(dp, p.dim, j, n, tid, post);
-      if (dg) store8<true>(dg, p.dim, j, n, tid, acc[j]);
+      if (dp && item != static_cast<int>(blockIdx.x)) load8<A != Access::Elements>(dp, p.dim, j, n, tid, post);
+      gate_gradient<A, W>(p, gate, j, n, tid, acc[j], post);
+      if (dp) store_partial<A>(dp, p.dim, j, n, tid, post);
+      if (p.part_gate)
+        store_partial<A>(p.part_gate + static_cast<int64_t>(item) * p.pitch, p.dim, j, n, tid, acc[j]);
+      else if (p.dgate)
+        store_row<A>(static_cast<float*>(p.dgate) + item / chunks * p.ld_dgate, p.dim, j, n, tid, acc[j]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = f2(0.0f);
     }
@@ -616,20 +712,21 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     if (p.part_post && PER_TOKEN)
-      store8<true>(p.part_post + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc[j]);
-    if (p.part_pre) store8<true>(p.part_pre + static_cast<int64_t>(blockIdx.x) * p.dim, p.dim, j, n, tid, acc_pre[j]);
+      store_partial<A>(p.part_post + static_cast<int64_t>(blockIdx.x) * p.pitch, p.dim, j, n, tid, acc[j]);
+    if (p.part_pre) store_partial<A>(p.part_pre + static_cast<int64_t>(blockIdx.x) * p.pitch, p.dim, j, n, tid, acc_pre[j]);
   }
   if (tid == 0) ring.drain();
 }
 
 // out[g][c] = sum over the group's `count` consecutive rows of part. A block
-// sums 32 columns, four a thread, over 32 row lanes, always in the same order;
+// sums 32 columns, four a thread, over 32 row lanes, always in the same order
+// (rows are padded to whole words);
 // four rows a lane are on their way at once. blockIdx.z picks one of three sums.
 struct Sums {
   const float* part[3];
   float* out[3];
   int64_t count[3], groups[3], ld_out[3];
-  int dim;
+  int dim, pitch;
 };
 constexpr int kSumThreads = 256;
 __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const Sums p) {
@@ -639,16 +736,11 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const Sums p) {
   allow_next_launch();
   if (!p.out[z]) return;
   const int c = blockIdx.x * 32 + threadIdx.x % 8 * 4, lane = threadIdx.x / 8;
-  const bool whole = p.dim % 4 == 0;
   for (int64_t g = blockIdx.y; g < p.groups[z]; g += gridDim.y) {
-    const float* part = p.part[z] + g * p.count[z] * p.dim + c;
+    const float* part = p.part[z] + g * p.count[z] * p.pitch + c;
     float4 v = make_float4(0, 0, 0, 0);
     auto add = [&](const float4& a) { v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w; };
-    auto row = [&](int64_t r) {
-      const float* at = part + r * p.dim;
-      if (whole) return *reinterpret_cast<const float4*>(at);
-      return make_float4(at[0], c + 1 < p.dim ? at[1] : 0.0f, c + 2 < p.dim ? at[2] : 0.0f, c + 3 < p.dim ? at[3] : 0.0f);
-    };
+    auto row = [&](int64_t r) { return *reinterpret_cast<const float4*>(part + r * p.pitch); };
     if (c < p.dim)
       for (int64_t r = lane; r < p.count[z]; r += 4 * 32) {
         float4 a[4];
@@ -735,18 +827,20 @@ Stream forward_stream(int dim, size_t elem) {
 
 // The backward pass. Its grid depends on the sizes alone, so that the scratch
 // for the blocks' sums does too.
-Stream backward_stream(int dim, size_t elem) {
+Stream backward_stream(int dim, size_t elem, bool aligned) {
   const int vecs = (dim + 7) / 8;
   Stream s{};
   s.nv = vecs <= 64 ? 1 : 2;
   s.threads = block_threads(dim, s.nv);
   s.per_sm = std::max(1u, std::min(8u, 512 / s.threads));
-  const size_t slot = 4 * static_cast<size_t>(dim) * elem, factors = 64 * static_cast<size_t>(s.nv) * s.threads;
+  const size_t slot = 4 * static_cast<size_t>(row_room(aligned, dim, static_cast<uint32_t>(elem)));
+  const size_t factors = 64 * static_cast<size_t>(s.nv) * s.threads;
   const size_t room = kSmemOfSm / s.per_sm;
   s.stages = static_cast<unsigned>(room > factors ? std::min<size_t>(kMaxRing, (room - factors) / slot) : 0);
   s.smem = s.stages * slot + factors;
   return s;
 }
+int padded(int64_t dim) { return static_cast<int>((dim + 7) / 8 * 8); }
 
 // How the backward pass splits its tokens: items of one gate row each, at
 // most `chunks` items per gate row, walked by `grid` blocks.
@@ -757,7 +851,7 @@ struct Split {
 };
 Split split_tokens(const rns8_cuda_residual_norm_backward_desc& d, int sm_count) {
   Split s;
-  const Stream st = backward_stream(static_cast<int>(d.dim), type_size(d.type));
+  const Stream st = backward_stream(static_cast<int>(d.dim), type_size(d.type), true);
   const int64_t target = static_cast<int64_t>(st.per_sm) * sm_count;
   s.per_token = d.gate && d.groups == d.tokens;
   s.groups = (s.per_token || !d.gate) ? 1 : d.groups;
@@ -785,12 +879,13 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, c
   p.x_out = d.x_out, p.h = d.h, p.q = d.q, p.q_scale = d.q_scale;
   p.scale = d.scale, p.eps = d.eps, p.offset = d.weight_offset, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
+  p.q_words = reinterpret_cast<uintptr_t>(d.q) % 8 == 0 && d.ld_q % 8 == 0;
   const size_t e = type_size(d.type), w = type_size(d.weight_type);
   const bool aligned = d.dim % 8 == 0 && aligned_rows(d.x, d.ld_x, e) && aligned_rows(d.y, d.ld_y, e) &&
                        aligned_rows(d.post_weight, 0, w) && aligned_rows(d.pre_weight, 0, w) &&
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.x_out, d.ld_x_out, e) &&
                        aligned_rows(d.h, d.ld_h, e) &&
-                       (!d.q || (reinterpret_cast<uintptr_t>(d.q) % 8 == 0 && d.ld_q % 8 == 0));
+                       (!d.q || p.q_words);
   // Below some four tokens an SM each block has one or two rows and nothing to
   // run ahead for: the direct form's shorter start wins.
   if (aligned && p.dim <= 16384 && d.tokens >= 4 * static_cast<int64_t>(sm_count)) {
@@ -809,11 +904,13 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, c
                        : launch_stream(t, wt, std::integral_constant<int, 2>{});
     });
   }
-  // Element by element a thread has eight times the accesses: more threads.
-  const int vecs = (p.dim + 7) / 8, vectors = aligned ? row_vectors(d.tokens, vecs) : (vecs <= kMaxThreads ? 1 : 4);
+  const int vectors = row_vectors(d.tokens, (p.dim + 7) / 8);
   return dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     constexpr int NV = decltype(nv)::value;
-    return launch_chained(residual_norm_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
+    constexpr Access A = decltype(al)::value                      ? Access::Words
+                         : NV == 1 && sizeof(decltype(t)) == 4 ? Access::Elements
+                                                               : Access::Shifted;
+    return launch_chained(residual_norm_kernel<decltype(t), decltype(wt), A, NV>,
                           dim3(static_cast<unsigned>(d.tokens)), block_threads(p.dim, NV), 0, 1, stream, p);
   });
 }
@@ -824,7 +921,7 @@ uint64_t residual_norm_backward_scratch_bytes(const rns8_cuda_residual_norm_back
   if (d.d_post) rows += s.grid;
   if (d.d_pre) rows += s.grid;
   if (gate_partials(d, s)) rows += s.items;
-  return rows * static_cast<uint64_t>(d.dim) * sizeof(float) + (rows ? 16 : 0);
+  return rows * static_cast<uint64_t>(padded(d.dim)) * sizeof(float) + (rows ? 16 : 0);
 }
 
 cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& d, int sm_count, cudaStream_t stream) {
@@ -835,6 +932,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   p.dxo = d.d_x_out, p.dh = d.pre_weight ? d.d_h : nullptr, p.x = d.x_out, p.y = d.y;
   p.post = d.post_weight, p.pre = d.pre_weight, p.gate = d.gate;
   p.dx = d.d_x, p.dy = d.d_y, p.dgate = d.gate ? d.d_gate : nullptr;
+  p.tokens = d.tokens, p.pitch = padded(d.dim);
   p.items = s.items, p.chunks = s.chunks, p.rows_per_item = s.rows_per_item, p.rows_per_group = s.rows_per_group;
   p.rows_per_gate = d.gate ? d.tokens / d.groups : 1;
   p.per_token = s.per_token;
@@ -844,11 +942,11 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   float* next = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(d.scratch) + 15) & ~uintptr_t(15));
   auto take = [&](int64_t rows) {
     float* at = next;
-    next += rows * d.dim;
+    next += rows * p.pitch;
     return at;
   };
   Sums sums{};
-  sums.dim = p.dim;
+  sums.dim = p.dim, sums.pitch = p.pitch;
   if (d.d_post) {
     p.part_post = take(s.grid);
     sums.part[0] = p.part_post, sums.out[0] = d.d_post, sums.count[0] = s.grid, sums.groups[0] = 1;
@@ -870,30 +968,33 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
                        aligned_rows(d.d_y, d.ld_d_y, e) &&
                        aligned_rows(d.d_gate, d.ld_d_gate, s.per_token ? e : sizeof(float));
-  const Stream st = backward_stream(p.dim, e);
-  // A block with one narrow row gains nothing from the ring and waits for its
-  // copies (us: 16 x 2048 direct 6.9, streamed 8.3; 16 x 8192 19.3 and 15.4).
-  const bool streamed = aligned && p.dim <= 8192 && st.stages > 0 && !(d.tokens < sm_count && p.dim <= 2048);
-  const int vectors = (p.dim + 7) / 8 <= kMaxThreads ? 1 : 4;
-  auto launch_stream = [&](auto t, auto wt, auto nv, auto per_token) {
-    auto kernel =
-        residual_norm_backward_stream_kernel<decltype(t), decltype(wt), decltype(nv)::value, decltype(per_token)::value>;
-    static std::atomic<uint64_t> configured{0};
-    const cudaError_t bad = raise_smem_limit_once(kernel, static_cast<int>(kSmemOfSm), configured);
-    if (bad != cudaSuccess) return bad;
-    return launch_chained(kernel, dim3(static_cast<unsigned>(s.grid)), st.threads, st.smem, 1, stream, p, st.stages);
-  };
-  cudaError_t err = streamed ? dispatch_types(d.type, d.weight_type, [&](auto t, auto wt) {
-    auto go = [&](auto nv) {
-      return s.per_token ? launch_stream(t, wt, nv, std::true_type{}) : launch_stream(t, wt, nv, std::false_type{});
-    };
-    return st.nv == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
-  }) : dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
+  const Stream st = backward_stream(p.dim, e, aligned);
+  // A block with one row gains nothing from the ring and waits for its copies
+  // (us, a gate row a token: 250 x 2048 f16 direct 8.4, streamed 11.0; 590 x
+  // 2048 f32 19.2 and 22.3; 290 x 4096 f16 15.8 and 14.8). Where rows start
+  // anywhere the words around them must lie within the matrix.
+  const bool one_row = d.tokens <= static_cast<int64_t>(st.per_sm) * sm_count;
+  const bool streamed = p.dim <= 8192 && (aligned || p.dim >= 8) && !(one_row && p.dim <= kNarrow);
+  const int vectors = streamed ? st.nv : p.dim <= kNarrow ? 1 : 4;
+  const cudaError_t launched = dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
+    using T = decltype(t);
+    using W = decltype(wt);
     constexpr int NV = decltype(nv)::value;
-    return launch_chained(residual_norm_backward_kernel<decltype(t), decltype(wt), decltype(al)::value, NV>,
-                          dim3(static_cast<unsigned>(s.grid)), block_threads(p.dim, NV), 0, 1, stream, p);
+    if (!streamed)
+      return launch_chained(residual_norm_backward_kernel<T, W, al ? Access::Words : Access::Shifted, NV == 2 ? 1 : NV>,
+                            dim3(static_cast<unsigned>(s.grid)), block_threads(p.dim, NV), 0, 1, stream, p);
+    auto go = [&](auto per_token) {
+      auto kernel = residual_norm_backward_stream_kernel<T, W, al ? Access::Words : Access::Elements, std::min(NV, 2),
+                                                       decltype(per_token)::value>;
+      static std::atomic<uint64_t> configured{0};
+      const cudaError_t bad = raise_smem_limit_once(kernel, static_cast<int>(kSmemOfSm), configured);
+      if (bad != cudaSuccess) return bad;
+      return launch_chained(kernel, dim3(static_cast<unsigned>(s.grid)), st.threads, st.smem, 1, stream, p, st.stages);
+    };
+    return s.per_token ? go(std::true_type{}) : go(std::false_type{});
   });
-  if (err != cudaSuccess) return err;
+  if (launched != cudaSuccess) return launched;
+  cudaError_t err = cudaSuccess;
   if (sums.out[0] || sums.out[1] || sums.out[2]) {
     const unsigned gy = static_cast<unsigned>(std::min<int64_t>(sums.out[2] ? s.groups : 1, 1024));
     err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), kSumThreads, 0, 1, stream, sums);
