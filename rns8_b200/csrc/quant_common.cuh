@@ -5,8 +5,9 @@
 // A row kernel gives every thread NV vectors of 8 elements. With ALIGNED rows
 // (whole vectors, base and leading dimension on 16-byte boundaries) vector v of
 // thread t covers elements 8 * (v * threads + t) .. + 7 and moves as 16-byte
-// words; otherwise its e-th element is (8 v + e) * threads + t, so that a
-// warp's element-wise accesses are contiguous. Elements past the row read as
+// words, as do rows that start anywhere, shifted into place; where rows go
+// element by element its e-th is (8 v + e) * threads + t, so that a warp's
+// accesses are contiguous. Elements past the row read as
 // zero. No kernel holds both forms: short calls wait for their code to arrive
 // as much as for their data.
 #pragma once
