@@ -719,33 +719,40 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
 }
 
 // out[g][c] = sum over the group's `count` consecutive rows of part. A block
-// sums 32 columns, four a thread, over 32 row lanes, always in the same order
-// (rows are padded to whole words);
-// four rows a lane are on their way at once. blockIdx.z picks one of three sums.
+// sums 32 columns, four a thread, over the rows that THREADS / 8 row lanes take
+// in turn, always in the same order (rows are padded to whole words); four rows
+// a lane are on their way at once. blockIdx.y picks the sum: the first two have
+// one group, the blocks after them walk the third's.
 struct Sums {
   const float* part[3];
   float* out[3];
-  int64_t count[3], groups[3], ld_out[3];
+  int64_t count[3], groups, ld_out;
   int dim, pitch;
 };
-constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const Sums p) {
-  __shared__ float4 s[kSumThreads / 32][8];
-  const int z = blockIdx.z;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) sum_rows_kernel(const Sums p) {
+  __shared__ float4 s[THREADS / 32][8];
+  constexpr int ROWS = THREADS / 8;
   wait_previous_launch();
   allow_next_launch();
-  if (!p.out[z]) return;
+  const bool third = blockIdx.y >= 2;
+  float* out = third ? p.out[2] : blockIdx.y ? p.out[1] : p.out[0];
+  if (!out) return;
+  const float* base = third ? p.part[2] : blockIdx.y ? p.part[1] : p.part[0];
+  const int count = static_cast<int>(third ? p.count[2] : blockIdx.y ? p.count[1] : p.count[0]);
+  const int64_t groups = third ? p.groups : 1, step = third ? gridDim.y - 2 : 1;
   const int c = blockIdx.x * 32 + threadIdx.x % 8 * 4, lane = threadIdx.x / 8;
-  for (int64_t g = blockIdx.y; g < p.groups[z]; g += gridDim.y) {
-    const float* part = p.part[z] + g * p.count[z] * p.pitch + c;
+  for (int64_t g = third ? blockIdx.y - 2 : 0; g < groups; g += step) {
+    const float* part = base + g * count * p.pitch + c;
     float4 v = make_float4(0, 0, 0, 0);
     auto add = [&](const float4& a) { v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w; };
-    auto row = [&](int64_t r) { return *reinterpret_cast<const float4*>(part + r * p.pitch); };
     if (c < p.dim)
-      for (int64_t r = lane; r < p.count[z]; r += 4 * 32) {
+      for (int r = lane; r < count; r += 4 * ROWS) {
         float4 a[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = r + i * 32 < p.count[z] ? row(r + i * 32) : make_float4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i)
+          a[i] = r + i * ROWS < count ? *reinterpret_cast<const float4*>(part + static_cast<int64_t>(r + i * ROWS) * p.pitch)
+                                      : make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) add(a[i]);
       }
@@ -758,8 +765,8 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const Sums p) {
     if (threadIdx.x < 32 && blockIdx.x * 32 + threadIdx.x < p.dim) {
       float all = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kSumThreads / 32; ++w) all += reinterpret_cast<const float*>(s[w])[threadIdx.x];
-      p.out[z][g * p.ld_out[z] + blockIdx.x * 32 + threadIdx.x] = all;
+      for (int w = 0; w < THREADS / 32; ++w) all += reinterpret_cast<const float*>(s[w])[threadIdx.x];
+      out[g * p.ld_out + blockIdx.x * 32 + threadIdx.x] = all;
     }
     __syncthreads();
   }
@@ -949,16 +956,16 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   sums.dim = p.dim, sums.pitch = p.pitch;
   if (d.d_post) {
     p.part_post = take(s.grid);
-    sums.part[0] = p.part_post, sums.out[0] = d.d_post, sums.count[0] = s.grid, sums.groups[0] = 1;
+    sums.part[0] = p.part_post, sums.out[0] = d.d_post, sums.count[0] = s.grid;
   }
   if (d.d_pre) {
     p.part_pre = take(s.grid);
-    sums.part[1] = p.part_pre, sums.out[1] = d.d_pre, sums.count[1] = s.grid, sums.groups[1] = 1;
+    sums.part[1] = p.part_pre, sums.out[1] = d.d_pre, sums.count[1] = s.grid;
   }
   if (gate_partials(d, s)) {
     p.part_gate = take(s.items);
     sums.part[2] = p.part_gate, sums.out[2] = static_cast<float*>(d.d_gate);
-    sums.count[2] = s.chunks, sums.groups[2] = s.groups, sums.ld_out[2] = d.ld_d_gate;
+    sums.count[2] = s.chunks, sums.groups = s.groups, sums.ld_out = d.ld_d_gate;
   }
 
   const size_t e = type_size(d.type), w = type_size(d.weight_type);
@@ -970,7 +977,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.d_gate, d.ld_d_gate, s.per_token ? e : sizeof(float));
   const Stream st = backward_stream(p.dim, e, aligned);
   // A block with one row gains nothing from the ring and waits for its copies
-  // (us, a gate row a token: 250 x 2048 f16 direct 8.4, streamed 11.0; 590 x
+  // (us, a gate row a token: 250 x 2048 f16 direct 8.4, streamed 10.9; 590 x
   // 2048 f32 19.2 and 22.3; 290 x 4096 f16 15.8 and 14.8). Where rows start
   // anywhere the words around them must lie within the matrix.
   const bool one_row = d.tokens <= static_cast<int64_t>(st.per_sm) * sm_count;
@@ -996,8 +1003,15 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   if (launched != cudaSuccess) return launched;
   cudaError_t err = cudaSuccess;
   if (sums.out[0] || sums.out[1] || sums.out[2]) {
-    const unsigned gy = static_cast<unsigned>(std::min<int64_t>(sums.out[2] ? s.groups : 1, 1024));
-    err = launch_chained(sum_rows_kernel, dim3((p.dim + 31) / 32, gy, 3), kSumThreads, 0, 1, stream, sums);
+    const unsigned walkers = sums.out[2] ? static_cast<unsigned>(std::min<int64_t>(s.groups, 1024)) : 0;
+    const dim3 grid((p.dim + 31) / 32, 2 + walkers);
+    // Few columns leave SMs idle unless blocks are wide, many groups do not (us,
+    // pass with its sums, 512 and 256 threads: 2000 x 1024 bf16 16.6 and 24.1,
+    // with 10 gate rows 2000 x 2048 22.5 and 25.0, 2000 x 8192 58.7 and 52.3).
+    if (grid.x * grid.y <= 8u * sm_count)
+      err = launch_chained(sum_rows_kernel<512>, grid, 512, 0, 1, stream, sums);
+    else
+      err = launch_chained(sum_rows_kernel<256>, grid, 256, 0, 1, stream, sums);
   }
   return err;
 }
