@@ -225,6 +225,11 @@ __device__ __forceinline__ bool copied(int64_t t, int64_t tokens) {
   return A == Access::Words || (t > 0 && t < tokens - 1);
 }
 
+// Asks for whole 16-byte words of global memory to be brought into L2.
+__device__ __forceinline__ void prefetch_l2(const void* words, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(words), "r"(bytes) : "memory");
+}
+
 // A ring of `stages` slots, each room for ROWS rows, filled by one thread's bulk
 // copies of the 16-byte words around them. A wait that runs out cannot be reported (these calls
 // have no status word), so it does not change the result instead: the thread
@@ -523,9 +528,10 @@ __global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_
 // lasts, in shared memory (a thread reads back its own, conflict-free); the
 // registers hold the row and two sums a channel. NV vectors a thread keep what
 // a row costs besides its elements (one reduction of six sums) small.
-// With a gate row per token (PER_TOKEN) the gate's words are read beside the
-// token's, and the factors kept are those of the weights alone.
-template <typename T, typename W, Access A, int NV, bool PER_TOKEN>
+// With a gate row per token (PER_TOKEN) the gate's words are copied with the
+// token's (GATE_COPIED) or brought to L2 with them, and the factors kept are
+// those of the weights alone.
+template <typename T, typename W, Access A, int NV, bool PER_TOKEN, bool GATE_COPIED>
 __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(const Backward p, uint32_t stages) {
   extern __shared__ __align__(16) uint8_t ring_bytes[];
   __shared__ __align__(8) uint64_t full[kMaxRing];
@@ -533,9 +539,10 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
   const int n = blockDim.x, tid = threadIdx.x;
   clear_slots(slots[0]);
   clear_slots(slots[1]);
-  RowRing<4> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)), row_room(A == Access::Words, p.dim, sizeof(T)),
-                   stages};
-  float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * 4 * ring.room);  // [NV][4][n]: a, a, pre, pre
+  constexpr int ROWS = GATE_COPIED ? 5 : 4;
+  RowRing<ROWS> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)),
+                     row_room(A == Access::Words, p.dim, sizeof(T)), stages};
+  float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * ROWS * ring.room);  // [NV][4][n]: a, a, pre, pre
   if (tid == 0) {
     for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
@@ -569,9 +576,16 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
   const int64_t lds[4] = {p.ld_dxo, p.ld_dh, p.ld_x, p.ld_y};
   auto fill = [&](uint32_t s, int64_t t) {
     const bool copy = copied<A>(t, p.tokens);
-    const uint8_t* rows[4];
+    const uint8_t* rows[ROWS];
 #pragma unroll
     for (int r = 0; r < 4; ++r) rows[r] = reinterpret_cast<const uint8_t*>(bases[r] && copy ? bases[r] + t * lds[r] : nullptr);
+    if (GATE_COPIED)
+      rows[ROWS - 1] = reinterpret_cast<const uint8_t*>(copy ? static_cast<const W*>(p.gate) + t * p.ld_gate : nullptr);
+    if (PER_TOKEN && copy && !GATE_COPIED) {
+      const W* gate = static_cast<const W*>(p.gate) + t * p.ld_gate;
+      prefetch_l2(reinterpret_cast<const uint8_t*>(gate) - row_offset(gate),
+                  (row_offset(gate) + p.dim * static_cast<uint32_t>(sizeof(W)) + 15) & ~15u);
+    }
     ring.fill(s, rows);
   };
   Cursor ahead{static_cast<int>(blockIdx.x), 0, 0};
@@ -614,10 +628,12 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
     const int64_t t = now.t;
     if (fresh) keep_factors(now.t);
     Raw8<W> gate_row[PER_TOKEN ? NV : 1];
-    if (PER_TOKEN)
+    auto take_gate = [&](const W* row) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        gate_row[j] = load_raw<A>(static_cast<const W*>(p.gate) + t * p.ld_gate, p.dim, j, n, tid);
+      for (int j = 0; j < NV; ++j) gate_row[j] = load_raw<A>(row, p.dim, j, n, tid);
+    };
+    const W* token_gate = PER_TOKEN ? static_cast<const W*>(p.gate) + t * p.ld_gate : nullptr;
+    if (PER_TOKEN && !GATE_COPIED) take_gate(token_gate);
     ring.wait();
     Raw8<T> dxo[NV], dh[NV], x[NV], y[NV];
     auto take = [&](auto row) {
@@ -631,10 +647,13 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
       }
     };
     // Two branches, so that these are shared-memory loads.
-    if (!ring.lost && copied<A>(t, p.tokens))
+    if (!ring.lost && copied<A>(t, p.tokens)) {
       take([&](int r) { return reinterpret_cast<const T*>(ring.slot(ring.stage, r) + row_offset(bases[r] + t * lds[r])); });
-    else
+      if constexpr (GATE_COPIED) take_gate(reinterpret_cast<const W*>(ring.slot(ring.stage, 4) + row_offset(token_gate)));
+    } else {
       take([&](int r) { return bases[r] + t * lds[r]; });
+      if (GATE_COPIED) take_gate(token_gate);
+    }
     release_stage_reads();
     RowSums sums{};
 #pragma unroll
@@ -834,13 +853,13 @@ Stream forward_stream(int dim, size_t elem) {
 
 // The backward pass. Its grid depends on the sizes alone, so that the scratch
 // for the blocks' sums does too.
-Stream backward_stream(int dim, size_t elem, bool aligned) {
+Stream backward_stream(int dim, size_t elem, bool aligned, int rows) {
   const int vecs = (dim + 7) / 8;
   Stream s{};
   s.nv = vecs <= 64 ? 1 : 2;
   s.threads = block_threads(dim, s.nv);
   s.per_sm = std::max(1u, std::min(8u, 512 / s.threads));
-  const size_t slot = 4 * static_cast<size_t>(row_room(aligned, dim, static_cast<uint32_t>(elem)));
+  const size_t slot = rows * static_cast<size_t>(row_room(aligned, dim, static_cast<uint32_t>(elem)));
   const size_t factors = 64 * static_cast<size_t>(s.nv) * s.threads;
   const size_t room = kSmemOfSm / s.per_sm;
   s.stages = static_cast<unsigned>(room > factors ? std::min<size_t>(kMaxRing, (room - factors) / slot) : 0);
@@ -858,7 +877,7 @@ struct Split {
 };
 Split split_tokens(const rns8_cuda_residual_norm_backward_desc& d, int sm_count) {
   Split s;
-  const Stream st = backward_stream(static_cast<int>(d.dim), type_size(d.type), true);
+  const Stream st = backward_stream(static_cast<int>(d.dim), type_size(d.type), true, 4);
   const int64_t target = static_cast<int64_t>(st.per_sm) * sm_count;
   s.per_token = d.gate && d.groups == d.tokens;
   s.groups = (s.per_token || !d.gate) ? 1 : d.groups;
@@ -975,7 +994,11 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
                        aligned_rows(d.d_y, d.ld_d_y, e) &&
                        aligned_rows(d.d_gate, d.ld_d_gate, s.per_token ? e : sizeof(float));
-  const Stream st = backward_stream(p.dim, e, aligned);
+  // Per-token gate rows go through the ring too where two slots an SM remain (us:
+  // 16384 x 4096 bf16 221, read beside it 282; 2000 x 8192, one slot, 80 and 70).
+  Stream st = backward_stream(p.dim, e, aligned, 5);
+  const bool gate_copied = aligned && s.per_token && e == w && st.stages * st.per_sm >= 2;
+  if (!gate_copied) st = backward_stream(p.dim, e, aligned, 4);
   // A block with one row gains nothing from the ring and waits for its copies
   // (us, a gate row a token: 250 x 2048 f16 direct 8.4, streamed 10.9; 590 x
   // 2048 f32 19.2 and 22.3; 290 x 4096 f16 15.8 and 14.8). Where rows start
@@ -990,15 +1013,17 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
     if (!streamed)
       return launch_chained(residual_norm_backward_kernel<T, W, al ? Access::Words : Access::Shifted, NV == 2 ? 1 : NV>,
                             dim3(static_cast<unsigned>(s.grid)), block_threads(p.dim, NV), 0, 1, stream, p);
-    auto go = [&](auto per_token) {
+    auto go = [&](auto per_token, auto gate_copied) {
       auto kernel = residual_norm_backward_stream_kernel<T, W, al ? Access::Words : Access::Elements, std::min(NV, 2),
-                                                       decltype(per_token)::value>;
+                                                         decltype(per_token)::value, decltype(gate_copied)::value>;
       static std::atomic<uint64_t> configured{0};
       const cudaError_t bad = raise_smem_limit_once(kernel, static_cast<int>(kSmemOfSm), configured);
       if (bad != cudaSuccess) return bad;
       return launch_chained(kernel, dim3(static_cast<unsigned>(s.grid)), st.threads, st.smem, 1, stream, p, st.stages);
     };
-    return s.per_token ? go(std::true_type{}) : go(std::false_type{});
+    if constexpr (al && sizeof(T) == sizeof(W))
+      if (gate_copied) return go(std::true_type{}, std::true_type{});
+    return s.per_token ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
   });
   if (launched != cudaSuccess) return launched;
   cudaError_t err = cudaSuccess;
