@@ -1,0 +1,56 @@
+"""Gradients of residual_norm at the ends of its range: rows far larger or
+smaller than 1, eps of zero or near it, rows of zeros, infinities where a value
+takes no part, offsets without a weight. Formulas and error model are those of
+test_gpu_residual_norm; rows of each kernel form are among the shapes."""
+
+import pytest
+
+from test_gpu_quant_linear import rng
+from test_gpu_residual_norm import check_backward, make
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def quant():
+    from rns8_b200 import quant
+
+    return quant
+
+
+# (tokens, dim, groups): one row a block, aligned and not; the ring, aligned
+# and not, with shared gate rows and a row a token; wider than the ring's rows.
+FORMS = [(5, 96, 1), (5, 1001, 5), (1500, 256, 3), (1400, 1001, 1), (1300, 520, 1300), (1300, 515, 1300),
+         (3, 8200, 1), (2, 8199, 2)]
+
+
+def gradients(tokens, dim, dtype, seed=0):
+    g = rng(dim + seed)
+    return [torch.randn(tokens, dim, generator=g, device="cuda").to(dtype) for _ in range(2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rms,eps", [(1e16, 1e-6), (1e14, 1e-6), (1e-13, 0.0), (1e-15, 0.0), (1e-17, 0.0)])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_row_magnitudes(quant, tokens, dim, groups, rms, eps, dtype):
+    """The powers of 1/rms that the gradients hold are never formed by
+    themselves: the cube of 1e-14 or of 1e13 is outside the 32-bit range."""
+    for of in ("x", "y", "xy"):
+        t = make(tokens, dim, groups, dtype)
+        for k in of:
+            t[k] = (t[k].float() * (rms / 2)).to(dtype)
+        dxo, dh = gradients(tokens, dim, dtype)
+        check_backward(quant, t, dxo, dh, dtype, eps=eps)
+        check_backward(quant, t, None, dh, dtype, eps=eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_zero_rows_and_a_tiny_eps(quant, tokens, dim, groups, dtype):
+    t = make(tokens, dim, groups, dtype)
+    t["x"][0] = 0
+    t["y"][tokens // 2] = 0
+    dxo, dh = gradients(tokens, dim, dtype)
+    check_backward(quant, t, dxo, dh, dtype, eps=1e-30)
