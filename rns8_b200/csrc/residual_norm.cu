@@ -361,6 +361,11 @@ struct Backward {
   int64_t tokens, items, chunks, rows_per_item, rows_per_group, rows_per_gate;
   float scale, eps, offset, inv_dim;
   int dim, pitch;
+  // Elements of x and y that are read: what takes no part counts as zeros, an
+  // infinity in it would make a NaN of every product with 0 (x without a norm of
+  // it, y without a norm of it or a gate's gradient). A branch around the loads
+  // costs more (4000 x 8191 f32 197 us, 222).
+  int x_dim, y_dim;
   bool per_token;  // one gate row per token: d_gate is written token by token
 };
 
@@ -421,8 +426,8 @@ struct RowSums {
 // u = sigma y, and the means are of the gradients' size, so that no power of a
 // row factor is formed; rho^3 or sigma^2 mean(v u) leave the 32-bit range for
 // rows whose rms is past 1e13 or below 1e-13. Two products a pair of elements
-// more than with powers (us: 16384 x 4096 bf16 142.5, 140 with them; 8192 x 8192
-// 148 and 143.5; 2000 x 2048 f32 29.9 and 30.2).
+// more than with powers (us: 16384 x 4096 bf16 143, 140 with them; 8192 x 8192
+// 144 and 143.5; 4000 x 8191 171 and 168).
 struct RowFactors {
   F2 rho, minus_tn, sigma, minus_vu;  // 1/rms(x), -mean(t n), 1/rms(y), -mean(v u)
 };
@@ -437,13 +442,14 @@ __device__ __forceinline__ RowFactors row_factors(const Backward& p, const RowSu
 }
 __device__ __forceinline__ void row_gradients(const RowFactors& r, const F2 (&dxo)[4], const F2 (&dh)[4],
                                               const F2 (&x)[4], const F2 (&y)[4], const F2 (&a)[4], const F2 (&pre)[4],
-                                              F2 (&dx)[4], F2 (&dy)[4], F2 (&udx)[4], F2 (&acc_pre)[4]) {
+                                              F2 (&dx)[4], F2 (&dy)[4], F2 (&udx)[4], F2 (&acc_pre)[4], bool post) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const F2 n = r.rho * x[e], u = r.sigma * y[e];
     dx[e] = fma(r.rho, fma(r.minus_tn, n, dh[e] * pre[e]), dxo[e]);
     acc_pre[e] = fma(dh[e], n, acc_pre[e]);
-    dy[e] = r.sigma * fma(r.minus_vu, u, a[e] * dx[e]);
+    dy[e] = a[e] * dx[e];
+    if (post) dy[e] = r.sigma * fma(r.minus_vu, u, dy[e]);  // without a norm of y, no value of y (0 * infinity)
     udx[e] = u * dx[e];
   }
 }
@@ -478,8 +484,8 @@ __global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_
         F2 dxo[4], dh[4], x[4], y[4], a[4], pre[4];
       };
       auto load = [&](int j, Vec& v) {
-        load_row<A>(x, p.dim, j, n, tid, v.x);
-        load_row<A>(y, p.dim, j, n, tid, v.y);
+        load_row<A>(x, p.x_dim, j, n, tid, v.x);
+        load_row<A>(y, p.y_dim, j, n, tid, v.y);
         load_or<A>(dxo, 0.0f, p.dim, j, n, tid, v.dxo);
         load_or<A>(dh, 0.0f, p.dim, j, n, tid, v.dh);
         make_factors<A, W>(p, gate, j, n, tid, v.a, v.pre);
@@ -496,7 +502,7 @@ __global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_
       for (int j = 0; j < NV; ++j) {
         if (NV > 1) load(j, v);
         F2 dx[4], dy[4], udx[4];
-        row_gradients(r, v.dxo, v.dh, v.x, v.y, v.a, v.pre, dx, dy, udx, acc_pre[j]);
+        row_gradients(r, v.dxo, v.dh, v.x, v.y, v.a, v.pre, dx, dy, udx, acc_pre[j], p.post);
         store_row<A>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
         store_row<A>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
         if (p.per_token) {
@@ -647,8 +653,8 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
         dxo[j] = dh[j] = Raw8<T>{};
         if (dxo_base) dxo[j] = load_raw<A>(row(0), p.dim, j, n, tid);
         if (dh_base) dh[j] = load_raw<A>(row(1), p.dim, j, n, tid);
-        x[j] = load_raw<A>(row(2), p.dim, j, n, tid);
-        y[j] = load_raw<A>(row(3), p.dim, j, n, tid);
+        x[j] = load_raw<A>(row(2), p.x_dim, j, n, tid);
+        y[j] = load_raw<A>(row(3), p.y_dim, j, n, tid);
       }
     };
     // Two branches, so that these are shared-memory loads.
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
         if (PER_TOKEN)
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] = a[e] * gate_row[j].pair(e);
-        row_gradients(r, fdxo, fdh, fx, fy, a, pre, dx, dy, udx, acc_pre[j]);
+        row_gradients(r, fdxo, fdh, fx, fy, a, pre, dx, dy, udx, acc_pre[j], p.post);
       }
       store_row<A>(static_cast<T*>(p.dx) + t * p.ld_dx, p.dim, j, n, tid, dx);
       store_row<A>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
@@ -969,6 +975,8 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   p.per_token = s.per_token;
   p.scale = d.scale, p.eps = d.eps, p.offset = d.weight_offset, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
+  p.x_dim = d.pre_weight ? p.dim : 0;
+  p.y_dim = d.post_weight || d.d_gate ? p.dim : 0;
 
   float* next = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(d.scratch) + 15) & ~uintptr_t(15));
   auto take = [&](int64_t rows) {

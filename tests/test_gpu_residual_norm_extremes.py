@@ -54,3 +54,41 @@ def test_zero_rows_and_a_tiny_eps(quant, tokens, dim, groups, dtype):
     t["y"][tokens // 2] = 0
     dxo, dh = gradients(tokens, dim, dtype)
     check_backward(quant, t, dxo, dh, dtype, eps=1e-30)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_without_pre_weight_x_out_takes_no_part(quant, tokens, dim, groups, dtype):
+    """d_x is d_x_out then, whatever x_out holds."""
+    for post in (True, False):
+        t = make(tokens, dim, groups, dtype, pre=False, post=post)
+        dxo, _ = gradients(tokens, dim, dtype)
+        args = {k: t[k] for k in ("post_weight", "gate")}
+        want = quant.residual_norm_backward(dxo, None, t["x"], t["y"], **args)
+        assert torch.equal(want[0], dxo)
+        x = t["x"].clone()
+        x[0, dim // 2], x[1, 0], x[tokens - 1, dim - 1] = float("inf"), float("nan"), float("-inf")
+        for a, b in zip(quant.residual_norm_backward(dxo, None, x, t["y"], **args), want):
+            assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_without_post_weight_y_enters_the_gates_gradient_alone(quant, tokens, dim, groups, dtype):
+    dxo, dh = gradients(tokens, dim, dtype)
+    bad = [(0, dim // 2, float("inf")), (1, 0, float("nan")), (tokens - 1, dim - 1, float("-inf"))]
+    for gate in (True, False):
+        t = make(tokens, dim, groups, dtype, post=False, gate=gate)
+        args = {k: t[k] for k in ("pre_weight", "gate")}
+        want = quant.residual_norm_backward(dxo, dh, t["x"], t["y"], **args)
+        y = t["y"].clone()
+        for row, col, value in bad:
+            y[row, col] = value
+        got = quant.residual_norm_backward(dxo, dh, t["x"], y, **args)
+        for i in (0, 1, 3):
+            assert torch.equal(got[i], want[i]), i
+        if gate:
+            of = torch.zeros_like(want[4], dtype=torch.bool)
+            for row, col, _ in bad:
+                of[row // (tokens // groups), col] = True
+            assert not torch.isfinite(got[4][of]).any() and torch.equal(got[4][~of], want[4][~of])
