@@ -359,7 +359,10 @@ struct Backward {
   void *dx, *dy, *dgate;
   float *part_post, *part_pre, *part_gate;  // per-block sums [grid][pitch], per-item gate sums [items][pitch]
   int64_t tokens, items, chunks, rows_per_item, rows_per_group, rows_per_gate;
-  float scale, eps, offset, inv_dim;
+  // The offsets are added to a weight; of an absent one, read as zeros, they are
+  // the whole factor.
+  float scale, eps, pre_offset, inv_dim;
+  float post_offset;
   int dim, pitch;
   // Elements of x and y that are read: what takes no part counts as zeros, an
   // infinity in it would make a NaN of every product with 0 (x without a norm of
@@ -381,13 +384,13 @@ template <Access A, typename W>
 __device__ __forceinline__ void make_factors(const Backward& p, const W* gate, int j, int n, int tid, F2 (&a)[4],
                                              F2 (&pre)[4]) {
   F2 w[4], g[4];
-  load_or<A>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<A>(static_cast<const W*>(p.post), 0.0f, p.dim, j, n, tid, w);
   load_or<A>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
-  load_or<A>(static_cast<const W*>(p.pre), -p.offset, p.dim, j, n, tid, pre);
+  load_or<A>(static_cast<const W*>(p.pre), -p.pre_offset, p.dim, j, n, tid, pre);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    a[e] = f2(p.scale) * g[e] * (w[e] + f2(p.offset));
-    pre[e] = pre[e] + f2(p.offset);
+    a[e] = f2(p.scale) * g[e] * (w[e] + f2(p.post_offset));
+    pre[e] = pre[e] + f2(p.pre_offset);
   }
 }
 // u dx summed or single -> the gate's gradient in place, post's share added.
@@ -395,12 +398,12 @@ template <Access A, typename W>
 __device__ __forceinline__ void gate_gradient(const Backward& p, const W* gate, int j, int n, int tid, F2 (&udx)[4],
                                               F2 (&acc_post)[4]) {
   F2 w[4], g[4];
-  load_or<A>(static_cast<const W*>(p.post), 1.0f - p.offset, p.dim, j, n, tid, w);
+  load_or<A>(static_cast<const W*>(p.post), 0.0f, p.dim, j, n, tid, w);
   load_or<A>(p.gate ? gate : nullptr, 1.0f, p.dim, j, n, tid, g);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     acc_post[e] = fma(f2(p.scale) * g[e], udx[e], acc_post[e]);
-    udx[e] = f2(p.scale) * (w[e] + f2(p.offset)) * udx[e];
+    udx[e] = f2(p.scale) * (w[e] + f2(p.post_offset)) * udx[e];
   }
 }
 // A row needs one reduction: with a = scale * gate * (offset + post),
@@ -973,8 +976,10 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   p.items = s.items, p.chunks = s.chunks, p.rows_per_item = s.rows_per_item, p.rows_per_group = s.rows_per_group;
   p.rows_per_gate = d.gate ? d.tokens / d.groups : 1;
   p.per_token = s.per_token;
-  p.scale = d.scale, p.eps = d.eps, p.offset = d.weight_offset, p.dim = static_cast<int>(d.dim);
+  p.scale = d.scale, p.eps = d.eps, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
+  p.post_offset = d.post_weight ? d.weight_offset : 1.0f;
+  p.pre_offset = d.pre_weight ? d.weight_offset : 0.0f;
   p.x_dim = d.pre_weight ? p.dim : 0;
   p.y_dim = d.post_weight || d.d_gate ? p.dim : 0;
 

@@ -92,3 +92,17 @@ def test_without_post_weight_y_enters_the_gates_gradient_alone(quant, tokens, di
             for row, col, _ in bad:
                 of[row // (tokens // groups), col] = True
             assert not torch.isfinite(got[4][of]).any() and torch.equal(got[4][~of], want[4][~of])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [3e8, -1e30, 1e30])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_offset_belongs_to_a_weight(quant, tokens, dim, groups, offset, dtype):
+    """An absent weight is a factor of 1 whatever the offset."""
+    t = make(tokens, dim, groups, dtype, post=False, pre=False)
+    dxo, _ = gradients(tokens, dim, dtype)
+    for gate in (t["gate"], None):
+        want = quant.residual_norm_backward(dxo, None, t["x"], t["y"], gate=gate)
+        got = quant.residual_norm_backward(dxo, None, t["x"], t["y"], gate=gate, weight_offset=offset)
+        for a, b in zip(got, want):
+            assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
