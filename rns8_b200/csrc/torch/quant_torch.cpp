@@ -72,7 +72,9 @@ void expect(rns8_status status, const char* where) {
 }
 
 uint32_t* status_word(int device) {
-  static std::vector<uint32_t*> known;  // the words live as long as the process; the GIL guards this
+  // The words live as long as the process, one a device (device_status sees to
+  // that). The GIL guards the table: only the call below lets other threads run.
+  static std::vector<uint32_t*> known;
   if (device < static_cast<int>(known.size()) && known[device]) return known[device];
   PyObject* r = PyObject_CallFunction(status_address, "i", device);
   if (!r) throw AlreadySet{};

@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import threading
 from typing import NamedTuple
 
 import torch
@@ -47,6 +48,7 @@ class QuantizedRows(NamedTuple):
 
 
 _status: dict[int, torch.Tensor] = {}
+_status_lock = threading.RLock()
 
 
 def device_status(device: int = 0) -> torch.Tensor:
@@ -54,12 +56,18 @@ def device_status(device: int = 0) -> torch.Tensor:
     OR 0x100 into when a bounded device wait ran out. The first call on a device
     allocates it, so that call cannot be part of a stream capture."""
     word = _status.get(device)
-    if word is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the first product on a device cannot be captured: run one, or device_status(), before")
-        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
-        torch.cuda.current_stream(device).synchronize()  # other streams may use it next
-    return word
+    if word is not None:
+        return word
+    # One word for the process's life: the binding keeps its address, and an
+    # allocation lets other threads run.
+    with _status_lock:
+        if device not in _status:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first product on a device cannot be captured: run one, or device_status(), before")
+            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
+            torch.cuda.current_stream(device).synchronize()  # other streams may use it next
+            _status.setdefault(device, word)
+        return _status[device]
 
 
 def check_status(device: int = 0) -> None:
