@@ -76,8 +76,9 @@ def check_status(device: int = 0) -> None:
     torch.cuda.synchronize(device)
     word = device_status(device)
     bits = int(word.item())
-    word.zero_()
     if bits:
+        word.zero_()
+        torch.cuda.synchronize(device)  # a product on another stream may report from here on
         raise RuntimeError(f"a bounded device wait ran out (status 0x{bits:x})")
 
 

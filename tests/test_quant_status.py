@@ -46,3 +46,23 @@ def test_one_word_for_threads_that_ask_at_once(quant, monkeypatch):
     for t in threads:
         t.join()
     assert len(made) == 1 and all(w is made[0] for w in got)
+
+
+def test_check_clears_the_word_before_it_returns(quant, monkeypatch):
+    """The word is cleared on the GPU, in the order of one stream; a product on
+    another stream may report as soon as the check is over."""
+    did = []
+
+    class Word:
+        def item(self):
+            did.append("read")
+            return 0x100
+
+        def zero_(self):
+            did.append("clear")
+
+    monkeypatch.setitem(quant._status, 0, Word())
+    monkeypatch.setattr(quant.torch.cuda, "synchronize", lambda device: did.append("synchronize"))
+    with pytest.raises(RuntimeError, match="0x100"):
+        quant.check_status(0)
+    assert did == ["synchronize", "read", "clear", "synchronize"]
