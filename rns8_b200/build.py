@@ -5,9 +5,10 @@ sm_100a only (-gencode arch=compute_100a,code=sm_100a) and linked into
 rns8_b200/_build/librns8.so, which is what the Python bindings, the tests and
 bench.py load. Object files are rebuilt when a source or header is newer.
 
-Where torch is installed, the torch binding of the 8-bit operators
+Where torch with CUDA is installed, the torch binding of the 8-bit operators
 (csrc/torch/quant_torch.cpp) is compiled against it by the host compiler into
-rns8_b200/_build/_quant_torch.so; the library itself knows no torch.
+rns8_b200/_build/_quant_torch.so; the library itself knows no torch, and its
+build succeeds where the binding's does not.
 
     python -m rns8_b200.build [--force] [--ptxas-verbose]
 """
@@ -100,17 +101,24 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int | None = N
             raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     if ptxas_verbose:
         print("\n".join(logs))
-    build_torch_binding(force)
+    try:
+        build_torch_binding(force)
+    except RuntimeError as e:  # the library is whole without it
+        print(f"rns8_b200.quant is not available: {e}", file=sys.stderr)
     return LIB
 
 
 def build_torch_binding(force: bool = False) -> Path | None:
-    """Compile the torch binding; None where torch is not installed. It is built
-    again when its sources, torch or the Python it was built for change."""
+    """Compile the torch binding; None where there is nothing to compile it
+    against: no torch, one without CUDA, or no Python headers. It is built again
+    when its sources, torch or the Python it was built for change. A binding that
+    does not compile raises, and leaves none of an earlier build."""
     if importlib.util.find_spec("torch") is None:
         return None
     import torch
 
+    if torch.version.cuda is None or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return None
     root = Path(torch.__file__).resolve().parent
     stamp = BUILD / "_quant_torch.stamp"
     built_for = f"{torch.__version__} {sys.version}"
@@ -128,6 +136,7 @@ def build_torch_binding(force: bool = False) -> Path | None:
            "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
+        TORCH_LIB.unlink(missing_ok=True)
         raise RuntimeError(f"torch binding failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     stamp.write_text(built_for)
     return TORCH_LIB
