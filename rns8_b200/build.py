@@ -111,8 +111,8 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int | None = N
 def build_torch_binding(force: bool = False) -> Path | None:
     """Compile the torch binding; None where there is nothing to compile it
     against: no torch, one without CUDA, or no Python headers. It is built again
-    when its sources, torch or the Python it was built for change. A binding that
-    does not compile raises, and leaves none of an earlier build."""
+    when its sources, its command, torch or the Python it was built for change. A
+    binding that does not compile raises, and leaves none of an earlier build."""
     if importlib.util.find_spec("torch") is None:
         return None
     import torch
@@ -120,12 +120,6 @@ def build_torch_binding(force: bool = False) -> Path | None:
     if torch.version.cuda is None or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
         return None
     root = Path(torch.__file__).resolve().parent
-    stamp = BUILD / "_quant_torch.stamp"
-    built_for = f"{torch.__version__} {sys.version}"
-    newest = max(p.stat().st_mtime for p in (TORCH_SRC, INCLUDE / "rns8" / "rns8_quant.h"))
-    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == built_for
-            and TORCH_LIB.stat().st_mtime >= newest):
-        return TORCH_LIB
     compiler = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else "g++"
     cuda = Path(nvcc()).resolve().parents[1]
     include = [INCLUDE, root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
@@ -134,6 +128,13 @@ def build_torch_binding(force: bool = False) -> Path | None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in include),
            str(TORCH_SRC), "-o", str(TORCH_LIB), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python",
            "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    stamp = BUILD / "_quant_torch.stamp"
+    built_for = "\n".join([torch.__version__, sys.version, *cmd])
+    # The ABI version and the status codes are compiled in from the other headers.
+    newest = max(p.stat().st_mtime for p in (TORCH_SRC, *INCLUDE.glob("rns8/*.h")))
+    if (not force and TORCH_LIB.exists() and stamp.exists() and stamp.read_text() == built_for
+            and TORCH_LIB.stat().st_mtime >= newest):
+        return TORCH_LIB
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         TORCH_LIB.unlink(missing_ok=True)

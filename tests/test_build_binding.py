@@ -66,3 +66,21 @@ def test_no_binding_without_cuda_torch_or_python_headers(build, monkeypatch, tmp
         monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path / "nowhere")})
     assert build.build() == build.LIB and build.build_torch_binding(force=True) is None
     assert not build.runs
+
+
+@pytest.mark.parametrize("name", ["rns8_quant.h", "abi.h", "status.h"])
+def test_compiled_again_when_a_header_changes(build, name):
+    assert build.build_torch_binding() == build.TORCH_LIB and len(build.runs) == 1
+    assert build.build_torch_binding() == build.TORCH_LIB and len(build.runs) == 1
+    later = time.time() + 10
+    os.utime(build.INCLUDE / "rns8" / name, (later, later))
+    build.build_torch_binding()
+    assert len(build.runs) == 2
+
+
+def test_compiled_again_when_the_command_changes(build, monkeypatch):
+    build.build_torch_binding()
+    paths = build.sysconfig.get_paths()
+    monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {**paths, "include": paths["include"] + "/."})
+    build.build_torch_binding()
+    assert len(build.runs) == 2
