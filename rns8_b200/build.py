@@ -122,10 +122,12 @@ def build_torch_binding(force: bool = False) -> Path | None:
     root = Path(torch.__file__).resolve().parent
     compiler = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else "g++"
     cuda = Path(nvcc()).resolve().parents[1]
-    include = [INCLUDE, root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
-               sysconfig.get_paths()["include"], cuda / "include"]
-    cmd = [compiler, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in include),
+    # System headers: their warnings are not ours.
+    system = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+              sysconfig.get_paths()["include"], cuda / "include"]
+    cmd = [compiler, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wextra",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           *(a for i in system for a in ("-isystem", str(i))),
            str(TORCH_SRC), "-o", str(TORCH_LIB), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python",
            "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     stamp = BUILD / "_quant_torch.stamp"
@@ -139,6 +141,8 @@ def build_torch_binding(force: bool = False) -> Path | None:
     if res.returncode != 0:
         TORCH_LIB.unlink(missing_ok=True)
         raise RuntimeError(f"torch binding failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    if res.stderr.strip():
+        print(res.stderr, file=sys.stderr)
     stamp.write_text(built_for)
     return TORCH_LIB
 

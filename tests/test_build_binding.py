@@ -84,3 +84,18 @@ def test_compiled_again_when_the_command_changes(build, monkeypatch):
     monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {**paths, "include": paths["include"] + "/."})
     build.build_torch_binding()
     assert len(build.runs) == 2
+
+
+def test_warnings_of_the_bindings_own_code_are_shown(build, monkeypatch, capsys):
+    run = build.subprocess.run
+
+    def warn(cmd, **kwargs):
+        run(cmd, **kwargs)
+        return subprocess.CompletedProcess(cmd, 0, "", "quant_torch.cpp: warning: unused variable")
+
+    monkeypatch.setattr(build.subprocess, "run", warn)
+    build.build_torch_binding()
+    cmd = build.runs[0]
+    assert "-w" not in cmd and "-Wall" in cmd and f"-I{build.INCLUDE}" in cmd
+    assert all(not c.startswith("-I") or c == f"-I{build.INCLUDE}" for c in cmd)  # the rest are system headers
+    assert "unused variable" in capsys.readouterr().err
