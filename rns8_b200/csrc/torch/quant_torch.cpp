@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -367,10 +368,16 @@ NormArgs norm_args(D& d, const at::Tensor& x, const char* x_name, const at::Tens
 }
 
 bool wants_gradient(PyObject* o) { return o != Py_None && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad(); }
+// A dual tensor of forward-mode differentiation, which is independent of the
+// recording of gradients.
+bool has_tangent(PyObject* o) {
+  return o != Py_None && THPVariable_Check(o) && c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         THPVariable_Unpack(o)._fw_grad(/*level=*/0).defined();
+}
 
 // ---- residual_norm(x, y, post, pre, gate, scale, eps, offset, form) ----
-// form 0: (x_out, h), or None where a gradient is wanted (the caller records
-// it); 1: (x_out, h) whatever is wanted; 2: (x_out, q, q_scale).
+// form 0: (x_out, h), or None where a derivative is wanted (the caller records
+// it, or refuses); 1: (x_out, h) whatever is wanted; 2: (x_out, q, q_scale).
 PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 9);
@@ -378,9 +385,9 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (PyErr_Occurred()) throw AlreadySet{};
     const at::Tensor& x = tensor(a[0], "x");
     const at::Tensor& y = tensor(a[1], "y");
-    if (form == 0 && at::GradMode::is_enabled())
+    if (form == 0)
       for (int i = 0; i < 5; ++i)
-        if (wants_gradient(a[i])) Py_RETURN_NONE;
+        if ((at::GradMode::is_enabled() && wants_gradient(a[i])) || has_tangent(a[i])) Py_RETURN_NONE;
     auto d = header<rns8_cuda_residual_norm_desc>(0);
     const NormArgs r = norm_args(d, x, "x", y, a[2], a[3], a[4], a[5], a[6], a[7]);
     if (form == 2 && !d.pre_weight) type_error("pre_weight: needed for int8 rows");

@@ -184,9 +184,10 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor
     by the row's root mean square and multiplies by weight_offset + weight
     (post_weight for y, pre_weight for h). Without post_weight y enters as it
     is; without pre_weight h is None. gate is one row of channels or rows that
-    each serve an equal run of tokens. Gradients flow to every tensor."""
+    each serve an equal run of tokens. Gradients flow to every tensor;
+    forward-mode tangents are refused (NotImplementedError)."""
     out = _binding.residual_norm(x, y, post_weight, pre_weight, gate, scale, eps, weight_offset, 0)
-    if out is None:  # a gradient is wanted
+    if out is None:  # a derivative is wanted
         return _ResidualNorm.apply(x, y, post_weight, pre_weight, gate, scale, eps, weight_offset)
     return out
 
