@@ -16,6 +16,9 @@
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <vector>
@@ -194,6 +197,34 @@ void expect_args(Py_ssize_t got, Py_ssize_t want) {
   if (got != want) type_error("expected " + std::to_string(want) + " arguments");
 }
 
+bool wants_gradient(PyObject* o) { return o != Py_None && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad(); }
+// A dual tensor of forward-mode differentiation, which is independent of the
+// recording of gradients.
+bool has_tangent(PyObject* o) {
+  return o != Py_None && THPVariable_Check(o) && c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         THPVariable_Unpack(o)._fw_grad(/*level=*/0).defined();
+}
+
+// Operators without a derivative. Forward mode has none to give: refused before
+// the call. A gradient is refused where it is asked for, as by torch's own: the
+// results carry a function that raises, so that inference with parameters needs
+// no torch.no_grad().
+void expect_no_tangents(const char* name, std::initializer_list<PyObject*> inputs) {
+  for (PyObject* o : inputs)
+    if (has_tangent(o)) throw Refused{PyExc_NotImplementedError, std::string(name) + " has no forward-mode derivative"};
+}
+void mark_underivable(const char* name, std::initializer_list<PyObject*> inputs, std::initializer_list<at::Tensor> results) {
+  if (!at::GradMode::is_enabled()) return;
+  std::vector<at::Tensor> from;
+  for (PyObject* o : inputs)
+    if (wants_gradient(o)) from.push_back(THPVariable_Unpack(o));
+  if (from.empty()) return;
+  auto node = std::shared_ptr<torch::autograd::NotImplemented>(
+      new torch::autograd::NotImplemented(name, torch::autograd::collect_next_edges(from)), torch::autograd::deleteNode);
+  for (const at::Tensor& r : results)
+    if (r.defined() && r.is_floating_point()) torch::autograd::set_history(r, node);
+}
+
 // ---- bind(quantize, linear_scratch, linear, norm, backward_scratch, backward, check, status, oom) ----
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -219,6 +250,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     expect_args(n, 1);
     const at::Tensor& x = tensor(a[0], "x");
+    expect_no_tangents("quantize_rows", {a[0]});
     auto d = header<rns8_cuda_quantize_desc>(0);
     d.x_type = float_type(x.scalar_type(), "x");
     d.device_id = cuda_device(x, "x");
@@ -230,6 +262,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.x = r.data, d.q = static_cast<int8_t*>(q.data_ptr()), d.scale = static_cast<float*>(scale.data_ptr());
     d.stream = stream_of(d.device_id);
     expect(lib.quantize_rows(&d), "rns8_cuda_quantize_rows_device");
+    mark_underivable("quantize_rows", {a[0]}, {scale});
     return tuple_of({q, scale});
   });
 }
@@ -242,6 +275,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& x = tensor(a[0], "activations");
     const at::Tensor* x_scale = optional_tensor(a[1], "a_scale");
     const at::Tensor& w = tensor(a[2], "w");
+    expect_no_tangents("the int8 product", {a[0], a[1], a[3], a[4]});
     const bool gated = a[5] == Py_True, quantize = a[7] == Py_True;
     const int device = cuda_device(x, "activations");
     auto d = header<rns8_cuda_linear_desc>(device);
@@ -299,6 +333,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       d.stream = stream_of(device);
       expect(lib.linear(&d), "rns8_cuda_linear_device");
     }
+    mark_underivable("the int8 product", {a[0], a[1], a[3], a[4]}, {quantize ? out_scale : out});
     return quantize ? tuple_of({out, out_scale}) : THPVariable_Wrap(out);
   });
 }
@@ -367,13 +402,6 @@ NormArgs norm_args(D& d, const at::Tensor& x, const char* x_name, const at::Tens
   return n;
 }
 
-bool wants_gradient(PyObject* o) { return o != Py_None && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad(); }
-// A dual tensor of forward-mode differentiation, which is independent of the
-// recording of gradients.
-bool has_tangent(PyObject* o) {
-  return o != Py_None && THPVariable_Check(o) && c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
-         THPVariable_Unpack(o)._fw_grad(/*level=*/0).defined();
-}
 
 // ---- residual_norm(x, y, post, pre, gate, scale, eps, offset, form) ----
 // form 0: (x_out, h), or None where a derivative is wanted (the caller records
@@ -388,6 +416,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (form == 0)
       for (int i = 0; i < 5; ++i)
         if ((at::GradMode::is_enabled() && wants_gradient(a[i])) || has_tangent(a[i])) Py_RETURN_NONE;
+    if (form == 2) expect_no_tangents("residual_norm_quantized", {a[0], a[1], a[2], a[3], a[4]});
     auto d = header<rns8_cuda_residual_norm_desc>(0);
     const NormArgs r = norm_args(d, x, "x", y, a[2], a[3], a[4], a[5], a[6], a[7]);
     if (form == 2 && !d.pre_weight) type_error("pre_weight: needed for int8 rows");
@@ -403,7 +432,9 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     d.ld_x = r.x.ld, d.x = r.x.data, d.x_out = x_out.data_ptr();
     if (d.tokens) expect(lib.norm(&d), "rns8_cuda_residual_norm_device");
-    return form == 2 ? tuple_of({x_out, q, s}) : tuple_of({x_out, h});
+    if (form != 2) return tuple_of({x_out, h});
+    mark_underivable("residual_norm_quantized", {a[0], a[1], a[2], a[3], a[4]}, {x_out, s});
+    return tuple_of({x_out, q, s});
   });
 }
 
@@ -413,6 +444,7 @@ PyObject* residual_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     expect_args(n, 10);
     const at::Tensor& x = tensor(a[2], "x_out");
     const at::Tensor& y = tensor(a[3], "y");
+    expect_no_tangents("residual_norm_backward", {a[0], a[1], a[2], a[3], a[4], a[5], a[6]});
     auto d = header<rns8_cuda_residual_norm_backward_desc>(0);
     const NormArgs r = norm_args(d, x, "x_out", y, a[4], a[5], a[6], a[7], a[8], a[9]);
     d.ld_x_out = r.x.ld, d.x_out = r.x.data;
@@ -453,6 +485,7 @@ PyObject* residual_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       d.scratch = scratch.data_ptr();
     }
     expect(lib.norm_backward(&d), "rns8_cuda_residual_norm_backward_device");
+    mark_underivable("residual_norm_backward", {a[0], a[1], a[2], a[3], a[4], a[5], a[6]}, {d_x, d_y, d_post, d_pre, d_gate});
     return tuple_of({d_x, d_y, d_post, d_pre, d_gate});
   });
 }

@@ -13,8 +13,9 @@ include/rns8/rns8_quant.h, whose entry points these functions call. Work is
 enqueued on the current stream of the tensors' device; nothing synchronises.
 Inputs made on another stream are the caller's to order and to keep alive
 (Tensor.record_stream), as for any torch operator. Leading dimensions of an
-activation are its tokens. residual_norm alone records gradients; the int8
-operators are for inference. Bad arguments raise ValueError or TypeError before
+activation are its tokens. residual_norm alone has a derivative; the others are
+for inference: asking for a gradient through their results raises RuntimeError,
+a forward-mode tangent among their inputs NotImplementedError. Bad arguments raise ValueError or TypeError before
 anything is enqueued; a refusal by the library raises api.Error.
 """
 
@@ -196,5 +197,5 @@ def residual_norm_quantized(x: torch.Tensor, y: torch.Tensor, *, pre_weight: tor
                             post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                             scale: float = 1.0, eps: float = 1e-6, weight_offset: float = 0.0):
     """(x_out, q, q_scale): residual_norm with h quantised per row as
-    quantize_rows does, from its unrounded values. For inference: no gradient."""
+    quantize_rows does, from its unrounded values. For inference: no derivative."""
     return _binding.residual_norm(x, y, post_weight, pre_weight, gate, scale, eps, weight_offset, 2)

@@ -28,3 +28,68 @@ def test_residual_norm_refuses_forward_mode(quant, name, grad_mode):
         t[name] = fwAD.make_dual(t[name], torch.ones_like(t[name]))
         with pytest.raises(NotImplementedError):
             quant.residual_norm(**t)
+
+
+def calls(quant, change):
+    """Name -> the operator's results with one input changed by change."""
+    a, s, w, ws, b = operands(4, 32, 64, 1)
+    x = torch.randn(4, 64, generator=rng(2), device="cuda")
+    t = make(4, 64, 2, torch.float32)
+    g = [torch.randn(4, 64, generator=rng(3), device="cuda") for _ in range(2)]
+    weights = {k: t[k] for k in ("post_weight", "pre_weight", "gate")}
+    back = lambda **k: quant.residual_norm_backward(*g, t["x"], **{"y": t["y"], **weights, **k})  # noqa: E731
+    found = {
+        "quantize_rows": lambda: quant.quantize_rows(change(x)),
+        "linear x": lambda: quant.linear(change(x), w, ws, bias=b),
+        "linear w_scale": lambda: quant.linear(x, w, change(ws)),
+        "linear bias": lambda: quant.linear(x, w, ws, bias=change(b)),
+        "linear to int8": lambda: quant.linear(change(x), w, ws, quantize=True)[:2],
+        "gemm_scaled a_scale": lambda: quant.gemm_scaled(a, change(s), w, ws),
+        "gemm_scaled bias, gated": lambda: quant.gemm_scaled(a, s, w, ws, bias=change(b), gated=True)[:2],
+    }
+    for k in t:
+        found[f"residual_norm_quantized {k}"] = lambda k=k: quant.residual_norm_quantized(**{**t, k: change(t[k])})
+    for k in ("y", "post_weight", "pre_weight", "gate"):
+        found[f"residual_norm_backward {k}"] = lambda k=k: back(**{k: change(t[k])})
+    found["residual_norm_backward d_h"] = lambda: quant.residual_norm_backward(g[0], change(g[1]), t["x"], t["y"], **weights)
+    return found
+
+
+def results(value):
+    return [r for r in (value if isinstance(value, tuple) else (value,)) if r is not None]
+
+
+def test_a_gradient_through_the_others_raises(quant):
+    """The values are those without autograd; asking for a gradient through
+    them is an error, where before the results were constants."""
+    plain, marked = calls(quant, lambda v: v), calls(quant, lambda v: v.clone().requires_grad_())
+    for name in plain:
+        want, got = results(plain[name]()), results(marked[name]())
+        floats = [r for r in got if r.is_floating_point()]
+        assert floats and all(r.requires_grad for r in floats), name
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), name
+        assert not any(r.requires_grad for r in want), name
+        for r in floats:
+            with pytest.raises(RuntimeError, match="not implemented"):
+                r.sum().backward()
+        with torch.no_grad():
+            assert not any(r.requires_grad for r in results(marked[name]())), name
+
+
+def test_the_others_refuse_forward_mode(quant):
+    for name in calls(quant, lambda v: v):
+        with fwAD.dual_level():
+            call = calls(quant, lambda v: fwAD.make_dual(v, torch.ones_like(v)))[name]
+            with pytest.raises(NotImplementedError):
+                call()
+
+
+def test_a_chain_of_products_carries_it(quant):
+    """Through int8 rows the scales carry the mark."""
+    _, _, w, ws, _ = operands(1, 64, 64, 1)
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    y = quant.linear(quant.linear(x, w, ws, quantize=True), w, ws)
+    assert y.requires_grad
+    with pytest.raises(RuntimeError, match="not implemented"):
+        y.sum().backward()
