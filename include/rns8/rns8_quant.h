@@ -142,13 +142,15 @@ RNS8_API rns8_status rns8_cuda_residual_norm_device(const rns8_cuda_residual_nor
  *   d_post = sum over tokens of d_p * u, d_pre = sum over tokens of d_h * n
  *   d_gate[g] = sum over the group's tokens of scale * p * d_x
  * d_x and d_y have `type`; d_post, d_pre and d_gate are 32-bit, except that a
- * gate of one row per token (groups == tokens) has d_gate in `type`. Any of
- * the last three may be NULL. Sums over tokens run in a fixed order: equal
+ * gate of one row per token (groups == tokens) has d_gate in `type`, unless
+ * RNS8_CUDA_NORM_D_GATE_F32 asks for 32 bits there too (a 32-bit gate's gradient
+ * then keeps its precision; weight_type F32 only). Any of the last three may be NULL. Sums over tokens run in a fixed order: equal
  * calls give equal bits. d_x may be d_x_out and d_y may be d_h. */
+#define RNS8_CUDA_NORM_D_GATE_F32 2u
 typedef struct rns8_cuda_residual_norm_backward_desc {
   uint64_t struct_size;
   uint32_t abi_version;
-  uint32_t flags; /* must be zero */
+  uint32_t flags; /* RNS8_CUDA_NORM_D_GATE_F32 or zero */
   int32_t device_id;
   uint32_t type;
   uint32_t weight_type;

@@ -65,8 +65,8 @@ rns8_status check_linear(const rns8_cuda_linear_desc* d) {
 
 // Types, sizes and parameters shared by the forward and backward descriptors.
 template <typename D>
-bool valid_norm(const D& d) {
-  if (d.flags || !float_type(d.type) || (d.weight_type != d.type && d.weight_type != RNS8_CUDA_TYPE_F32)) return false;
+bool valid_norm(const D& d, uint32_t flags) {
+  if ((d.flags & ~flags) || !float_type(d.type) || (d.weight_type != d.type && d.weight_type != RNS8_CUDA_TYPE_F32)) return false;
   if (d.tokens < 0 || d.tokens > kMaxExtent || d.dim < 1 || d.dim > 32768) return false;
   if (!(d.eps >= 0.0f) || d.eps > 3.4e38f) return false;
   const uint32_t w = type_size(d.weight_type);
@@ -78,7 +78,9 @@ bool valid_norm(const D& d) {
 }
 
 bool valid_backward(const rns8_cuda_residual_norm_backward_desc& d) {
-  if (!valid_norm(d) || !aligned_to(d.d_post, 4) || !aligned_to(d.d_pre, 4)) return false;
+  if (!valid_norm(d, RNS8_CUDA_NORM_D_GATE_F32) || !aligned_to(d.d_post, 4) || !aligned_to(d.d_pre, 4)) return false;
+  const bool gate_f32 = d.flags & RNS8_CUDA_NORM_D_GATE_F32;
+  if (gate_f32 && d.weight_type != RNS8_CUDA_TYPE_F32) return false;
   if ((d.d_post && !d.post_weight) || (d.d_pre && !d.pre_weight) || (d.d_gate && !d.gate)) return false;
   if (d.tokens == 0) return !d.d_gate || (d.groups >= 0 && valid_rows(d.d_gate, d.groups, d.dim, d.ld_d_gate, 4));
   const uint32_t e = type_size(d.type);
@@ -87,7 +89,7 @@ bool valid_backward(const rns8_cuda_residual_norm_backward_desc& d) {
   if (!valid_rows(d.x_out, d.tokens, d.dim, d.ld_x_out, e) || !valid_rows(d.y, d.tokens, d.dim, d.ld_y, e) ||
       !valid_rows(d.d_x, d.tokens, d.dim, d.ld_d_x, e) || !valid_rows(d.d_y, d.tokens, d.dim, d.ld_d_y, e))
     return false;
-  return !d.d_gate || valid_rows(d.d_gate, d.groups, d.dim, d.ld_d_gate, d.groups == d.tokens ? e : 4);
+  return !d.d_gate || valid_rows(d.d_gate, d.groups, d.dim, d.ld_d_gate, d.groups == d.tokens && !gate_f32 ? e : 4);
 }
 
 }  // namespace
@@ -124,7 +126,7 @@ extern "C" rns8_status rns8_cuda_linear_device(const rns8_cuda_linear_desc* desc
 }
 
 extern "C" rns8_status rns8_cuda_residual_norm_device(const rns8_cuda_residual_norm_desc* desc) {
-  if (!valid_header(desc) || !valid_norm(*desc)) return RNS8_INVALID_ARGUMENT;
+  if (!valid_header(desc) || !valid_norm(*desc, 0)) return RNS8_INVALID_ARGUMENT;
   const auto& d = *desc;
   if (!d.pre_weight && (d.h || d.q)) return RNS8_INVALID_ARGUMENT;
   if (d.pre_weight && !d.h && !d.q && d.tokens > 0) return RNS8_INVALID_ARGUMENT;

@@ -370,6 +370,7 @@ struct Backward {
   // costs more (4000 x 8191 f32 197 us, 222).
   int x_dim, y_dim;
   bool per_token;  // one gate row per token: d_gate is written token by token
+  bool dgate_f32;  // in 32 bits then too (W of 32 bits only)
 };
 
 // What the two backward forms share, for one vector of a row.
@@ -405,6 +406,14 @@ __device__ __forceinline__ void gate_gradient(const Backward& p, const W* gate, 
     acc_post[e] = fma(f2(p.scale) * g[e], udx[e], acc_post[e]);
     udx[e] = f2(p.scale) * (w[e] + f2(p.post_offset)) * udx[e];
   }
+}
+// A token's own gate gradient.
+template <Access A, typename T, typename W>
+__device__ __forceinline__ void store_token_gate(const Backward& p, int64_t t, int j, int n, int tid, const F2 (&v)[4]) {
+  if constexpr (sizeof(T) < sizeof(W)) {
+    if (p.dgate_f32) return store_row<A>(static_cast<float*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, v);
+  }
+  store_row<A>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, v);
 }
 // A row needs one reduction: with a = scale * gate * (offset + post),
 // mean(v u) expands over dx = dxo + rho (t - mean(t n) n) into sums that do
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_
         store_row<A>(static_cast<T*>(p.dy) + t * p.ld_dy, p.dim, j, n, tid, dy);
         if (p.per_token) {
           gate_gradient<A, W>(p, gate, j, n, tid, udx, acc_post[j]);
-          if (p.dgate) store_row<A>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+          if (p.dgate) store_token_gate<A, T, W>(p, t, j, n, tid, udx);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
@@ -714,7 +723,7 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
           acc[j][e] = fma(f2(p.scale) * gate_row[j].pair(e), udx[e], acc[j][e]);
           udx[e] = base[e] * udx[e];
         }
-        if (p.dgate) store_row<A>(static_cast<T*>(p.dgate) + t * p.ld_dgate, p.dim, j, n, tid, udx);
+        if (p.dgate) store_token_gate<A, T, W>(p, t, j, n, tid, udx);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + udx[e];
@@ -976,6 +985,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   p.items = s.items, p.chunks = s.chunks, p.rows_per_item = s.rows_per_item, p.rows_per_group = s.rows_per_group;
   p.rows_per_gate = d.gate ? d.tokens / d.groups : 1;
   p.per_token = s.per_token;
+  p.dgate_f32 = d.flags & RNS8_CUDA_NORM_D_GATE_F32;
   p.scale = d.scale, p.eps = d.eps, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
   p.post_offset = d.post_weight ? d.weight_offset : 1.0f;
@@ -1011,7 +1021,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
                        aligned_rows(d.post_weight, 0, w) && aligned_rows(d.pre_weight, 0, w) &&
                        aligned_rows(d.gate, d.ld_gate, w) && aligned_rows(d.d_x, d.ld_d_x, e) &&
                        aligned_rows(d.d_y, d.ld_d_y, e) &&
-                       aligned_rows(d.d_gate, d.ld_d_gate, s.per_token ? e : sizeof(float));
+                       aligned_rows(d.d_gate, d.ld_d_gate, s.per_token && !p.dgate_f32 ? e : sizeof(float));
   // Per-token gate rows go through the ring too where two slots an SM remain (us:
   // 16384 x 4096 bf16 221, read beside it 282; 2000 x 8192, one slot, 80 and 70).
   Stream st = backward_stream(p.dim, e, aligned, 5);

@@ -476,7 +476,10 @@ PyObject* residual_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       d.d_pre = static_cast<float*>(d_pre.data_ptr());
     }
     if (r.gate_tensor) {
-      d_gate = empty(r.gate_tensor->sizes(), d.groups == d.tokens ? x.scalar_type() : at::kFloat, device);
+      const bool per_token = d.groups == d.tokens;
+      if (per_token && d.weight_type == RNS8_CUDA_TYPE_F32 && d.type != RNS8_CUDA_TYPE_F32)
+        d.flags |= RNS8_CUDA_NORM_D_GATE_F32;
+      d_gate = empty(r.gate_tensor->sizes(), per_token && !d.flags ? x.scalar_type() : at::kFloat, device);
       d.d_gate = d_gate.data_ptr();
     }
     d.scratch_bytes = lib.norm_backward_scratch(&d);

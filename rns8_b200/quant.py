@@ -147,8 +147,8 @@ def residual_norm_backward(d_x_out: torch.Tensor | None, d_h: torch.Tensor | Non
                            weight_offset: float = 0.0):
     """(d_x, d_y, d_post_weight, d_pre_weight, d_gate) of residual_norm from the
     gradients of its two results, its first result x_out and its input y. The
-    sums over tokens are 32-bit; d_gate is x's type where the gate has one row
-    per token. Entries without their input are None."""
+    sums over tokens are 32-bit; the d_gate of a gate in x's type with one row
+    per token is in that type. Entries without their input are None."""
     return _binding.residual_norm_backward(d_x_out, d_h, x_out, y, post_weight, pre_weight, gate, scale, eps,
                                            weight_offset)
 

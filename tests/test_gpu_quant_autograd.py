@@ -4,7 +4,7 @@ them or says that it cannot, the others never drop one silently."""
 import pytest
 
 from test_gpu_quant_linear import operands, rng
-from test_gpu_residual_norm import make
+from test_gpu_residual_norm import EPS32, backward_ref, close, make
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,24 @@ def test_a_chain_of_products_carries_it(quant):
     assert y.requires_grad
     with pytest.raises(RuntimeError, match="not implemented"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,dim", [(1, 64), (5, 1001), (1300, 520), (1300, 515), (3, 8200)])
+def test_a_32_bit_gate_has_a_32_bit_gradient(quant, tokens, dim, dtype):
+    """With a row a token too, and for one token: it was rounded to the
+    activations' 16 bits, so its precision depended on the batch."""
+    t = make(tokens, dim, tokens, dtype, torch.float32)
+    g = rng(dim)
+    dxo, dh = (torch.randn(tokens, dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+    args = {k: t[k] for k in ("y", "post_weight", "pre_weight", "gate")}
+    got = quant.residual_norm_backward(dxo, dh, t["x"], **args, scale=0.7, eps=1e-5)
+    value, terms = backward_ref(dxo, dh, t["x"], **args, scale=0.7, eps=1e-5, offset=0.0)[4]
+    assert got[4].dtype == torch.float32
+    close(got[4], value, 257 * EPS32 * terms, torch.float32)
+    gate = t["gate"].clone().requires_grad_()
+    xo, h = quant.residual_norm(**{**t, "gate": gate})
+    torch.autograd.backward([xo, h], [dxo, dh])
+    want = quant.residual_norm_backward(dxo, dh, xo.detach(), t["y"], post_weight=t["post_weight"],
+                                        pre_weight=t["pre_weight"], gate=t["gate"])[4]
+    assert torch.equal(gate.grad, want)

@@ -108,6 +108,22 @@ def test_norm_backward_refusals(rns8, change):
     assert rns8.lib().rns8_cuda_residual_norm_backward_device(packed) == INVALID
     assert rns8.lib().rns8_cuda_residual_norm_backward_scratch_bytes(packed) == 0
 
+def test_norm_backward_gate_gradient_type(rns8):
+    """32 bits on request, for a 32-bit gate; ld and address go by that type."""
+    base = dict(weight_type=2, scale=1.0, eps=1e-6, tokens=6, dim=10, groups=6, ld_d_x_out=10, ld_x_out=10, ld_y=10,
+                ld_gate=10, ld_d_x=10, ld_d_y=10, ld_d_gate=10, d_x_out=P, x_out=P, y=P, post_weight=P, gate=P, d_x=P,
+                d_y=P, d_post=P, d_gate=P)
+
+    def need(**change):
+        return rns8.lib().rns8_cuda_residual_norm_backward_scratch_bytes(
+            descriptor("ResidualNormBackwardDesc", rns8, base, change))
+
+    assert need() > 0 and need(flags=2) > 0  # scratch for d_post: the descriptor is valid
+    assert need(d_gate=P + 2) > 0 and need(flags=2, d_gate=P + 2) == 0
+    assert need(flags=2, weight_type=0) == 0 and need(flags=3) == 0 and need(flags=4) == 0
+    d = norm_desc(rns8, flags=2)
+    assert rns8.lib().rns8_cuda_residual_norm_device(d) == INVALID
+
 
 def test_null_descriptors(rns8):
     for name in ("quantize_rows", "linear", "residual_norm", "residual_norm_backward"):
