@@ -100,6 +100,12 @@ typedef struct rns8_cuda_linear_desc {
  * scratch, scratch_bytes, status and stream do not); 0 for a malformed one. */
 RNS8_API uint64_t rns8_cuda_linear_scratch_bytes(const rns8_cuda_linear_desc* desc);
 RNS8_API rns8_status rns8_cuda_linear_device(const rns8_cuda_linear_desc* desc);
+/* The kernel that a call of this descriptor runs on a GPU of sm_count
+ * multiprocessors: tile = 0 with tokens on the tensor cores' lanes, else channels
+ * on lanes with `tile` tokens to a tile and `splits` blocks that share k. For
+ * profiles and for tests that are to cover every form. */
+RNS8_API rns8_status rns8_cuda_linear_form(const rns8_cuda_linear_desc* desc, int32_t sm_count, uint32_t* tile,
+                                           uint32_t* splits);
 
 /* The step between two blocks. With N(v) = v / sqrt(mean(v^2) + eps), all in
  * 32-bit floats and rounded once on output:

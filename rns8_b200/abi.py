@@ -311,10 +311,11 @@ SIGNATURES = {
     "rns8_cuda_ipc_open": (c_status, [C.c_int, vp, P(vp)]),
     "rns8_cuda_ipc_close": (c_status, [C.c_int, vp]),
     "rns8_cuda_wait_probe": (c_status, [C.c_int, u32, u64, vp, vp]),
-    # 8-bit operators (include/rns8/rns8_quant.h); each takes one descriptor
+    # 8-bit operators (include/rns8/rns8_quant.h); each takes a descriptor
     "rns8_cuda_quantize_rows_device": (c_status, [vp]),
     "rns8_cuda_linear_scratch_bytes": (u64, [vp]),
     "rns8_cuda_linear_device": (c_status, [vp]),
+    "rns8_cuda_linear_form": (c_status, [vp, C.c_int32, P(u32), P(u32)]),
     "rns8_cuda_residual_norm_device": (c_status, [vp]),
     "rns8_cuda_residual_norm_backward_scratch_bytes": (u64, [vp]),
     "rns8_cuda_residual_norm_backward_device": (c_status, [vp]),

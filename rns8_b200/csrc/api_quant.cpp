@@ -125,6 +125,17 @@ extern "C" rns8_status rns8_cuda_linear_device(const rns8_cuda_linear_desc* desc
   return launch_result(rns8cuda::linear(*desc, sm_count_of(desc->device_id), static_cast<cudaStream_t>(desc->stream)));
 }
 
+extern "C" rns8_status rns8_cuda_linear_form(const rns8_cuda_linear_desc* desc, int32_t sm_count, uint32_t* tile,
+                                             uint32_t* splits) {
+  const rns8_status c = check_linear(desc);
+  if (c != RNS8_SUCCESS) return c;
+  if (sm_count < 1 || desc->m < 1 || !tile || !splits) return RNS8_INVALID_ARGUMENT;
+  const rns8cuda::LinearForm f = rns8cuda::linear_form(*desc, sm_count);
+  *tile = f.tile;
+  *splits = f.splits;
+  return RNS8_SUCCESS;
+}
+
 extern "C" rns8_status rns8_cuda_residual_norm_device(const rns8_cuda_residual_norm_desc* desc) {
   if (!valid_header(desc) || !valid_norm(*desc, 0)) return RNS8_INVALID_ARGUMENT;
   const auto& d = *desc;

@@ -28,6 +28,7 @@
 #include "device_common.cuh"
 #include "gemm_internal.hpp"
 #include "linear_internal.hpp"
+#include "quant_kernels.hpp"
 #include "quant_common.cuh"
 #include "quant_launch.cuh"
 
@@ -631,6 +632,11 @@ Choice choose(int64_t m, int64_t n, int64_t total_kb, bool gated, int sm_count) 
 }
 
 }  // namespace
+
+LinearForm linear_form(const rns8_cuda_linear_desc& d, int sm_count) {
+  const Choice c = choose(d.m, d.n, (d.k + BK - 1) / BK, (d.flags & RNS8_CUDA_LINEAR_GATED) != 0, sm_count);
+  return LinearForm{c.tokens_on_lanes ? 0u : static_cast<uint32_t>(c.tile), c.splits};
+}
 
 cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
   TcLinear p{};

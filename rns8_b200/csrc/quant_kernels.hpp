@@ -17,6 +17,11 @@ cudaError_t quantize_rows(const void* x, uint32_t x_type, int64_t rows, int64_t 
                           int64_t ld_q, float* scale, cudaStream_t stream, const AlignRows* align = nullptr);
 
 uint64_t linear_scratch_bytes(const rns8_cuda_linear_desc& d);
+// Tokens to a tile and blocks to a cluster; tile 0: tokens on lanes.
+struct LinearForm {
+  uint32_t tile, splits;
+};
+LinearForm linear_form(const rns8_cuda_linear_desc& d, int sm_count);
 cudaError_t linear(const rns8_cuda_linear_desc& d, int sm_count, cudaStream_t stream);
 
 cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, cudaStream_t stream);
