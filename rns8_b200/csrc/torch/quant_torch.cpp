@@ -112,7 +112,7 @@ void expect_device(const at::Tensor& t, int device, const char* name) {
 }
 
 // A tensor as rows of its last dimension. `held` keeps the copy alive that a
-// tensor without such a view needs.
+// tensor without such a view, or whose rows share memory, needs.
 struct Rows {
   void* data;
   int64_t rows, cols, ld;
@@ -139,6 +139,11 @@ Rows rows_of(const at::Tensor& t, const char* name) {
   r.rows = two->size(0);
   if (r.cols > 1 && two->stride(1) != 1) value_error(std::string(name) + ": elements of a row must be contiguous");
   r.ld = r.rows > 1 ? two->stride(0) : std::max<int64_t>(r.cols, 1);
+  if (r.ld < r.cols) {  // rows that share memory, as of expand()
+    r.held = two->contiguous();
+    two = &r.held;
+    r.ld = r.cols;
+  }
   r.data = two->data_ptr();
   return r;
 }

@@ -13,10 +13,12 @@ include/rns8/rns8_quant.h, whose entry points these functions call. Work is
 enqueued on the current stream of the tensors' device; nothing synchronises.
 Inputs made on another stream are the caller's to order and to keep alive
 (Tensor.record_stream), as for any torch operator. Leading dimensions of an
-activation are its tokens. residual_norm alone has a derivative; the others are
-for inference: asking for a gradient through their results raises RuntimeError,
-a forward-mode tangent among their inputs NotImplementedError. Bad arguments raise ValueError or TypeError before
-anything is enqueued; a refusal by the library raises api.Error.
+activation are its tokens; rows that share memory (expand) are copied first.
+
+residual_norm alone has a derivative. The others are for inference: asking for a
+gradient through their results raises RuntimeError, a forward-mode tangent among
+their inputs NotImplementedError. Bad arguments raise ValueError or TypeError
+before anything is enqueued; a refusal by the library raises api.Error.
 """
 
 from __future__ import annotations
