@@ -1027,13 +1027,17 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   Stream st = backward_stream(p.dim, e, aligned, 5);
   const bool gate_copied = aligned && s.per_token && e == w && st.stages * st.per_sm >= 2;
   if (!gate_copied) st = backward_stream(p.dim, e, aligned, 4);
-  // A block with one row gains nothing from the ring and waits for its copies
-  // (us, a gate row a token, sums by blocks of 256 threads: 250 x 2048 f16 direct
-  // 8.4, streamed 10.9; 590 x 2048 f32 19.2 and 22.3; 290 x 4096 f16 15.8 and
-  // 14.8). Where rows start anywhere the words around them must lie within the
-  // matrix.
+  // A block with one row gains nothing from the ring and waits for its copies,
+  // unless direct blocks, one an SM past 2048 columns, would run in turns (us,
+  // direct and streamed, a gate row a token: 250 x 2048 f16 7.0 and 8.5; bf16 590 x
+  // 1024 8.4 and 10.1, 148 x 4096 7.4 and 10.0, but 200 x 4096 11.5 and 10.7, 440 x
+  // 2056 13.8 and 10.9). In turns too, floats on 16-byte boundaries (290 x 4096 16.9
+  // and 18.8) and 16-bit rows off them (290 x 4095 17.4 and 19.7) go direct, floats
+  // off them do not (440 x 2559 24.6 and 17.4). Where rows start anywhere the words
+  // around them must lie within the matrix.
   const bool one_row = d.tokens <= static_cast<int64_t>(st.per_sm) * sm_count;
-  const bool streamed = p.dim <= 8192 && (aligned || p.dim >= 8) && !(one_row && p.dim <= kNarrow);
+  const bool in_turns = p.dim > 2048 && d.tokens > sm_count && aligned == (e == 2);
+  const bool streamed = p.dim <= 8192 && (aligned || p.dim >= 8) && !(one_row && !in_turns && p.dim <= kNarrow);
   const int vectors = streamed ? st.nv : p.dim <= kNarrow ? 1 : 4;
   const cudaError_t launched = dispatch(d.type, d.weight_type, aligned, vectors, [&](auto t, auto wt, auto al, auto nv) {
     using T = decltype(t);

@@ -120,3 +120,15 @@ def test_backward(quant, tokens, dim, groups, dtype):
     got = check_backward(quant, t, dxo, dh, dtype)
     for a, b in zip(check_backward(quant, t, dxo, dh, dtype), got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("per_token", [False, True])
+@pytest.mark.parametrize("tokens,dim", [(148, 4096), (149, 4096), (290, 4096), (290, 4095), (440, 2056), (440, 2559),
+                                        (443, 2048), (296, 3080)])
+def test_backward_around_one_token_a_block(quant, tokens, dim, per_token, dtype):
+    """Either side of the choice between rows in registers and the ring."""
+    t = make(tokens, dim, tokens if per_token else 1, dtype)
+    g = rng(dim)
+    dxo, dh = (torch.randn(tokens, dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+    check_backward(quant, t, dxo, dh, dtype)
