@@ -47,7 +47,7 @@ class W8A8Block:
         post1, pre1, post2, pre2 = self.norms
         x1, q, s = quant.residual_norm_quantized(x, attention, post_weight=post1, pre_weight=pre1, gate=self.gates[0],
                                                  scale=self.scale)
-        hidden = quant.gemm_scaled(q, s, *self.gate_up, gated=True, out_dtype=x.dtype)
+        hidden = quant.gemm_scaled(q, s, *self.gate_up, gated=True, out_dtype=x.dtype, quantize=True)
         y = quant.linear(hidden, *self.down)
         return quant.residual_norm(x1, y, post_weight=post2, pre_weight=pre2, gate=self.gates[1], scale=self.scale)
 

@@ -120,9 +120,10 @@ def gemm_scaled(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale
     gated, w's first half are the gate's channels: silu(first) * second.
 
     The result is a tensor of out_dtype, or, with quantize, QuantizedRows made
-    from the 32-bit values: int8 in, int8 out, for a chain of products. A gated
-    product's result is the next product's tokens, so there quantize is the
-    default; pass quantize=False for a tensor."""
+    from the 32-bit values: int8 in, int8 out, for a chain of products, whose next
+    product then answers in out_dtype. quantize unset means: as the next step
+    takes it, QuantizedRows from a gated product, a tensor from any other. Say
+    quantize=True or False where the result's type matters to the caller."""
     if a_scale is None:
         raise TypeError("a_scale: expected a tensor")
     if quantize or (quantize is None and gated):
@@ -132,8 +133,9 @@ def gemm_scaled(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale
 
 def linear(x: torch.Tensor | QuantizedRows, w: torch.Tensor, w_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
            gated: bool = False, out_dtype: torch.dtype | None = None, quantize: bool = False):
-    """gemm_scaled(*quantize_rows(x), w, w_scale) in one call; the result has
-    x's type unless out_dtype is given. QuantizedRows go in as they are."""
+    """gemm_scaled(*quantize_rows(x), w, w_scale, quantize=quantize) in one call:
+    float rows in and, gated or not, a tensor out, in x's type unless out_dtype is
+    given; QuantizedRows with quantize. QuantizedRows go in as they are."""
     if isinstance(x, QuantizedRows):
         return gemm_scaled(x.q, x.scale, w, w_scale, bias=bias, gated=gated, out_dtype=out_dtype or x.dtype,
                            quantize=bool(quantize))
