@@ -183,6 +183,13 @@ RNS8_API uint64_t
 rns8_cuda_residual_norm_backward_scratch_bytes(const rns8_cuda_residual_norm_backward_desc* desc);
 RNS8_API rns8_status rns8_cuda_residual_norm_backward_device(const rns8_cuda_residual_norm_backward_desc* desc);
 
+/* The limit of these operators' bounded device waits in SM cycles, for every
+ * later call of the process: 1 to 4000000000, 0 for the usual one (the largest,
+ * about two seconds). A short one shows what a wait that runs out does: a product
+ * sets its status word where data was late, a norm reads the row from global
+ * memory instead (at 1, every row). */
+RNS8_API rns8_status rns8_cuda_quant_wait_limit(uint64_t cycles);
+
 #ifdef __cplusplus
 }
 #endif

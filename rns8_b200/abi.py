@@ -317,6 +317,7 @@ SIGNATURES = {
     "rns8_cuda_linear_device": (c_status, [vp]),
     "rns8_cuda_linear_form": (c_status, [vp, C.c_int32, P(u32), P(u32)]),
     "rns8_cuda_residual_norm_device": (c_status, [vp]),
+    "rns8_cuda_quant_wait_limit": (c_status, [u64]),
     "rns8_cuda_residual_norm_backward_scratch_bytes": (u64, [vp]),
     "rns8_cuda_residual_norm_backward_device": (c_status, [vp]),
 }

@@ -94,6 +94,17 @@ bool valid_backward(const rns8_cuda_residual_norm_backward_desc& d) {
 
 }  // namespace
 
+namespace {
+std::atomic<int64_t> wait_cycles{rns8cuda::kQuantWaitCycles};
+}  // namespace
+int64_t rns8cuda::quant_wait_cycles() { return wait_cycles.load(std::memory_order_relaxed); }
+
+extern "C" rns8_status rns8_cuda_quant_wait_limit(uint64_t cycles) {
+  if (cycles > static_cast<uint64_t>(rns8cuda::kQuantWaitCycles)) return RNS8_INVALID_ARGUMENT;
+  wait_cycles.store(cycles ? static_cast<int64_t>(cycles) : rns8cuda::kQuantWaitCycles, std::memory_order_relaxed);
+  return RNS8_SUCCESS;
+}
+
 extern "C" rns8_status rns8_cuda_quantize_rows_device(const rns8_cuda_quantize_desc* desc) {
   if (!valid_header(desc) || desc->flags || !float_type(desc->x_type)) return RNS8_INVALID_ARGUMENT;
   const auto& d = *desc;

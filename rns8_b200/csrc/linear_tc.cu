@@ -16,8 +16,9 @@
 //                     few tokens, where the weights' stream bounds it, and
 //                     shapes with fewer tiles than SMs.
 //
-// Every mbarrier wait is bounded; one that runs out sets the device status
-// word and the block drains its copies and products and exits.
+// Every mbarrier wait is bounded (by wait_cycles, those before a block leaves by
+// the full limit); one that runs out sets the device status word and the block
+// drains its copies and products and exits.
 #include <cuda.h>
 
 #include <algorithm>
@@ -48,6 +49,7 @@ struct __align__(64) TcLinear {
   uint32_t m_tiles, n_tiles, units;  // tokens on lanes
   uint32_t after_quantize, vector_rows;
   uint32_t* status;
+  int64_t wait_cycles;
 };
 
 __device__ __forceinline__ void report_timeout(const TcLinear& p, volatile int* abort_flag) {
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(Lanes<BN>::THREADS, Lanes<BN>::PER_SM) linear_
       for (uint32_t i = 0; i < early; ++i) load_tokens(i, kb0 + i);
       uint32_t pending = (1u << early) - 1, parities = 0, stage = early % STAGES, phase = early / STAGES;
       for (uint32_t kb = kb0 + early; kb < kb1; ++kb) {
-        if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u)) {
+        if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u, p.wait_cycles)) {
           if (!*abort_flag) report_timeout(p, abort_flag);
           break;
         }
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(Lanes<BN>::THREADS, Lanes<BN>::PER_SM) linear_
       constexpr uint32_t idesc = make_idesc_i8(LANES, BN, /*b_mn_major=*/false);
       uint32_t stage = 0, phase = 0;
       for (uint32_t kb = kb0; kb < kb1; ++kb) {
-        if (*abort_flag || !mbar_wait_bounded(&full[stage], phase)) {
+        if (*abort_flag || !mbar_wait_bounded(&full[stage], phase, p.wait_cycles)) {
           if (!*abort_flag) report_timeout(p, abort_flag);
           break;
         }
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(Lanes<BN>::THREADS, Lanes<BN>::PER_SM) linear_
   const bool direct = !GATED && splits == 1;
   int4* sums = reinterpret_cast<int4*>(smem);  // [BN / 4][LANES], once the stages are consumed
   if (warp >= 2) {
-    if (!mbar_wait_bounded(done, 0) && !*abort_flag) report_timeout(p, abort_flag);
+    if (!mbar_wait_bounded(done, 0, p.wait_cycles) && !*abort_flag) report_timeout(p, abort_flag);
     (void)epilogue_all<32 * L::WARPS>(true);  // the token scales are in place
     tc_fence_after();
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
         const int32_t w0 = static_cast<int32_t>(nt * COLS);
         const int32_t w1 = GATED ? static_cast<int32_t>(p.n + nt * COLS) : w0 + BN / 2;
         for (uint32_t kb = 0; kb < p.total_kb; ++kb) {
-          if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u)) {
+          if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1u, p.wait_cycles)) {
             if (!*abort_flag) report_timeout(p, abort_flag);
             ok = false;
             break;
@@ -449,13 +451,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       for (uint32_t u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-        if (*abort_flag || !mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u)) {
+        if (*abort_flag || !mbar_wait_bounded(&acc_empty[acc], acc_phase ^ 1u, p.wait_cycles)) {
           if (!*abort_flag) report_timeout(p, abort_flag);
           break;
         }
         tc_fence_after();
         for (uint32_t kb = 0; kb < p.total_kb; ++kb) {
-          if (*abort_flag || !mbar_wait_bounded(&full[stage], phase)) {
+          if (*abort_flag || !mbar_wait_bounded(&full[stage], phase, p.wait_cycles)) {
             if (!*abort_flag) report_timeout(p, abort_flag);
             ok = false;
             break;
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tokens_kernel(const __grid_
       const int64_t t = static_cast<int64_t>(mt) * LANES + quarter * 32 + lane;
       const bool token = t < p.m;
       const float s = token ? p.a_scale[t] : 0.0f;
-      const bool ok = !*abort_flag && mbar_wait_bounded(&acc_full[acc], acc_phase);
+      const bool ok = !*abort_flag && mbar_wait_bounded(&acc_full[acc], acc_phase, p.wait_cycles);
       if (!ok && !*abort_flag) report_timeout(p, abort_flag);
       // The column values are in place, and the four warps stop together or
       // not at all: the next tile's barrier needs all of them.
@@ -645,6 +647,7 @@ cudaError_t linear_tc(const LinearArgs& a, int sm_count, cudaStream_t stream) {
   p.total_kb = static_cast<uint32_t>((a.k + BK - 1) / BK);
   p.after_quantize = a.after_quantize;
   p.status = a.status;
+  p.wait_cycles = quant_wait_cycles();
   const size_t elem = a.out_type == RNS8_CUDA_TYPE_F32 ? 4 : 2;
   p.vector_rows = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ld_out * elem % 16 == 0;
   const int64_t w_rows = a.gated ? 2 * a.n : a.n;

@@ -10,6 +10,10 @@
 
 namespace rns8cuda {
 
+// The limit of the kernels' waits (rns8_cuda_quant_wait_limit), usual and now.
+constexpr int64_t kQuantWaitCycles = 4000000000;
+int64_t quant_wait_cycles();
+
 // With `align` the same launch also copies another int8 matrix's rows to
 // 16-byte boundaries (quant_common.cuh).
 struct AlignRows;

@@ -23,6 +23,7 @@ namespace rns8cuda {
 namespace {
 
 constexpr int kMaxThreads = 1024;
+static_assert(kQuantWaitCycles == kWaitBudgetCycles, "the limit that the kernels' last waits keep");
 
 struct Forward {
   int64_t rows_per_gate;
@@ -34,6 +35,7 @@ struct Forward {
   float scale, eps, offset, inv_dim;
   int dim;
   bool q_words;
+  int64_t wait_cycles;
 };
 
 // How a kernel reads and writes rows.
@@ -238,9 +240,11 @@ template <int ROWS>
 struct RowRing {
   uint8_t* base;
   uint64_t* full;
-  uint32_t row_bytes, room, stages, stage = 0, phase = 0;
+  uint32_t row_bytes, room, stages;
+  int64_t wait_cycles;
+  uint32_t stage = 0, phase = 0;
   uint32_t filled = 0, parity = ~0u;  // slots ever filled, parity of each one's last fill
-  bool lost = false;
+  bool lost = wait_cycles <= 1;  // one cycle is over before the first look
 
   __device__ uint8_t* slot(uint32_t s, int row) const { return base + (s * ROWS + row) * room; }
   // Bytes of the words around a row.
@@ -258,7 +262,7 @@ struct RowRing {
       if (rows[r]) bulk_load_1d(slot(s, r), rows[r] - row_offset(rows[r]), words(rows[r]), &full[s]);
   }
   __device__ void wait() {
-    if (!lost) lost = !mbar_wait_bounded(&full[stage], phase);
+    if (!lost) lost = !mbar_wait_bounded(&full[stage], phase, wait_cycles);
   }
   // The filling thread, last: its copies have landed before the block exits.
   __device__ void drain() const {
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_stream_kernel(const
   const int n = blockDim.x, tid = threadIdx.x;
   for (int b = 0; b < 4; ++b) clear_slots(slots[b / 2][b % 2]);
   const uint32_t row_bytes = p.dim * sizeof(T);
-  RowRing<2> ring{ring_bytes, full, row_bytes, row_bytes, stages};
+  RowRing<2> ring{ring_bytes, full, row_bytes, row_bytes, stages, p.wait_cycles};
   if (tid == 0) {
     for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
@@ -371,6 +375,7 @@ struct Backward {
   int x_dim, y_dim;
   bool per_token;  // one gate row per token: d_gate is written token by token
   bool dgate_f32;  // in 32 bits then too (W of 32 bits only)
+  int64_t wait_cycles;
 };
 
 // What the two backward forms share, for one vector of a row.
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(512) residual_norm_backward_stream_kernel(cons
   clear_slots(slots[1]);
   constexpr int ROWS = GATE_COPIED ? 5 : 4;
   RowRing<ROWS> ring{ring_bytes, full, static_cast<uint32_t>(p.dim * sizeof(T)),
-                     row_room(A == Access::Words, p.dim, sizeof(T)), stages};
+                     row_room(A == Access::Words, p.dim, sizeof(T)), stages, p.wait_cycles};
   float4* factors = reinterpret_cast<float4*>(ring_bytes + stages * ROWS * ring.room);  // [NV][4][n]: a, a, pre, pre
   if (tid == 0) {
     for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
@@ -928,6 +933,7 @@ cudaError_t residual_norm(const rns8_cuda_residual_norm_desc& d, int sm_count, c
   p.x_out = d.x_out, p.h = d.h, p.q = d.q, p.q_scale = d.q_scale;
   p.scale = d.scale, p.eps = d.eps, p.offset = d.weight_offset, p.dim = static_cast<int>(d.dim);
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
+  p.wait_cycles = quant_wait_cycles();
   p.q_words = reinterpret_cast<uintptr_t>(d.q) % 8 == 0 && d.ld_q % 8 == 0;
   const size_t e = type_size(d.type), w = type_size(d.weight_type);
   const bool aligned = d.dim % 8 == 0 && aligned_rows(d.x, d.ld_x, e) && aligned_rows(d.y, d.ld_y, e) &&
@@ -990,6 +996,7 @@ cudaError_t residual_norm_backward(const rns8_cuda_residual_norm_backward_desc& 
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
   p.post_offset = d.post_weight ? d.weight_offset : 1.0f;
   p.pre_offset = d.pre_weight ? d.weight_offset : 0.0f;
+  p.wait_cycles = quant_wait_cycles();
   p.x_dim = d.pre_weight ? p.dim : 0;
   p.y_dim = d.post_weight || d.d_gate ? p.dim : 0;
 
