@@ -475,7 +475,10 @@ constexpr int kNarrow = 4096;  // widest row of the direct backward form's block
 
 // A block walks items (runs of tokens that share a gate row) and keeps the
 // sums over tokens in registers: for dgate and dpost A = sum of u * dx over an
-// item (both are multiples of it by per-channel factors), for dpre its own.
+// item (both are multiples of it by per-channel factors), for dpre its own. With
+// NV = 4 (past 8192 columns) the registers of so many threads do not hold a
+// vector's values: 0.5 to 1.1 KB a thread spill, and the row is read twice (us:
+// 4096 x 16384 bf16 610, where HBM needs 125; 1000 x 16383 760).
 template <typename T, typename W, Access A, int NV>
 __global__ void __launch_bounds__(NV == 1 ? kNarrow / 8 : kMaxThreads) residual_norm_backward_kernel(const Backward p) {
   __shared__ SumSlots<6> slots[2];
