@@ -106,3 +106,25 @@ def test_offset_belongs_to_a_weight(quant, tokens, dim, groups, offset, dtype):
         got = quant.residual_norm_backward(dxo, None, t["x"], t["y"], gate=gate, weight_offset=offset)
         for a, b in zip(got, want):
             assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,dim,groups", FORMS)
+def test_bad_rows_stay_apart(quant, tokens, dim, groups, dtype):
+    """An infinity or NaN makes its own token's gradients NaN, as the formulas
+    do, and leaves every other token's bits."""
+    t = make(tokens, dim, groups, dtype)
+    args = {k: t[k] for k in ("post_weight", "pre_weight", "gate")}
+    dxo, dh = gradients(tokens, dim, dtype)
+    want = quant.residual_norm_backward(dxo, dh, t["x"], t["y"], **args)
+    for of in range(4):
+        rows = [v.clone() for v in (dxo, dh, t["x"], t["y"])]
+        rows[of][0, dim // 3], rows[of][tokens - 1, dim - 1] = float("nan"), float("inf")
+        got = quant.residual_norm_backward(*rows, **args)
+        for a, b in zip(got[:2], want[:2]):
+            assert torch.equal(a[1:tokens - 1], b[1:tokens - 1])
+        assert not torch.isfinite(got[1][[0, tokens - 1]]).any()  # d_y depends on all of its token
+        if of == 3:  # y reaches d_y and the gate, not d_x
+            assert torch.equal(got[0], want[0])
+        else:
+            assert not torch.isfinite(got[0][[0, tokens - 1]]).all(1).any()
